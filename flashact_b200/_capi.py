@@ -16,6 +16,7 @@ FA_KV_COMPACT_SPLIT_HALF, FA_KV_FLASHRT_INTERLEAVED = 0, 1
 EXPORTS = ["fa_create", "fa_pi05_load_weights", "fa_pi05_load_weights_q", "fa_ma2_load_weights", "fa_ma2_set_rope", "fa_set_modulation", "fa_bind_prefix_kv", "fa_bind_prefix_kv_masked", "fa_sample_actions",
            "fa_sync", "fa_set_stage_timing", "fa_get_stage_cycles", "fa_last_launch_count",
            "fa_set_fault_injection", "fa_debug_trace", "fa_pi05_modulations_noalloc", "fa_quantize_fp8_rows", "fa_quantize_nvfp4",
+           "fa_nvfp4_linear", "fa_kv8_append", "fa_kv8_read", "fa_kv8_attention_workspace", "fa_kv8_attention",
            "fa_last_error", "fa_destroy"]
 
 
@@ -57,6 +58,15 @@ class FaMa2Weights(ctypes.Structure):
     _fields_ = [(n, FaTensor) for n in MA2_WEIGHT_FIELDS]
 
 
+class FaKv8(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, ctypes.c_int) for n in ("batch", "layers", "heads", "head_dim", "capacity", "block")]
+
+
+class FaRows(ctypes.Structure):
+    _fields_ = [("ptr", ctypes.c_void_p)] + [(n, ctypes.c_longlong) for n in ("batch", "token", "head")]
+
+
 class FlashActError(RuntimeError):
     def __init__(self, status, msg):
         super().__init__(f"{STATUS_NAMES.get(status, status)}: {msg}")
@@ -76,6 +86,7 @@ def load_library(path: str = None) -> ctypes.CDLL:
     if not os.path.exists(path):
         raise FlashActError(FA_ERR_UNSUPPORTED, f"{path} missing: run `python -m flashact_b200.build`")
     lib = ctypes.CDLL(path)
+    KV, R, LL = ctypes.POINTER(FaKv8), ctypes.POINTER(FaRows), ctypes.c_longlong
     H, S, P, I = ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int
     sig = {
         "fa_create": (S, [I, ctypes.POINTER(FaConfig), I, ctypes.POINTER(ctypes.c_void_p)]),
@@ -96,6 +107,11 @@ def load_library(path: str = None) -> ctypes.CDLL:
         "fa_pi05_modulations_noalloc": (S, [ctypes.POINTER(FaPi05Weights), I, I, P, P, P]),
         "fa_quantize_fp8_rows": (S, [P, I, I, I, I, P, P, P]),
         "fa_quantize_nvfp4": (S, [P, I, I, I, I, P, P, P, P]),
+        "fa_nvfp4_linear": (S, [P, I, I, I, LL, P, P, P, P, I, P, LL, P]),
+        "fa_kv8_append": (S, [KV, I, I, R, R, I, P, P, P]),
+        "fa_kv8_read": (S, [KV, P, I, P, P, I, P]),
+        "fa_kv8_attention_workspace": (S, [KV, I, I, I, ctypes.POINTER(ctypes.c_size_t)]),
+        "fa_kv8_attention": (S, [KV, I, I, I, R, I, P, P, P, I, ctypes.c_float, I, R, P, ctypes.c_size_t, P]),
         "fa_last_error": (ctypes.c_char_p, [H]),
         "fa_destroy": (None, [H]),
     }

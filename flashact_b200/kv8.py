@@ -1,0 +1,167 @@
+"""A prefix KV cache in 8 bits (fa_kv8_* in include/flashact.h): E4M3 codes with a power-of-two scale for each
+block of tokens and head, half the bytes of the bf16 prefix that the action experts bind. Tokens are appended on
+the GPU, queries attend to them as they are, and bind_prefix_cache / bind_context_cache of the engines take the
+values. No CPU fallback."""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _capi as C
+from .pi05 import _DT
+
+
+def _bad(msg):
+    return C.FlashActError(C.FA_ERR_INVALID, msg)
+
+
+class Kv8Cache:
+    """K and V of `batch` observations, `layers` layers and `heads` key heads, up to `capacity` tokens (rounded up to
+    whole blocks). `lens` (int32 [batch], on the device) counts the tokens of each observation; it is changed by
+    advance() and by the caller, not by append(), so that every layer of a step appends at the same place."""
+
+    def __init__(self, batch: int, layers: int, heads: int, head_dim: int, capacity: int, *, block: int = 64,
+                 device: int | str | torch.device = 0):
+        dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        cap = -(-capacity // block) * block if block > 0 else capacity
+        shape = (batch, layers, heads)
+        if min(shape) < 1 or cap < 1:
+            raise _bad(f"a cache of batch, layers, heads = {shape} and {capacity} tokens")
+        self._own(torch.zeros(*shape, cap, head_dim, dtype=torch.uint8, device=dev),
+                  torch.zeros(*shape, head_dim, cap, dtype=torch.uint8, device=dev),
+                  torch.full((*shape, cap // block), 2.0 ** -96, device=dev),
+                  torch.full((*shape, cap // block), 2.0 ** -96, device=dev),
+                  torch.zeros(batch, dtype=torch.int32, device=dev))
+
+    @classmethod
+    def from_tensors(cls, k, v, k_scale, v_scale, *, lens=None):
+        """A cache over tensors that the caller owns, in the layout of fa_kv8: k uint8 [batch][layers][heads][capacity]
+        [head_dim], v uint8 [batch][layers][heads][head_dim][capacity], scales fp32 [batch][layers][heads][blocks],
+        lens int32 [batch]; contiguous, on one GPU."""
+        self = cls.__new__(cls)
+        self._own(k, v, k_scale, v_scale, torch.zeros(k.shape[0], dtype=torch.int32, device=k.device) if lens is None else lens)
+        return self
+
+    def _own(self, k, v, k_scale, v_scale, lens):
+        if k.dim() != 5 or v.dim() != 5 or k_scale.dim() != 4:
+            raise _bad("k and v have five dimensions, the scales four")
+        b, layers, heads, cap, d = k.shape
+        blocks = k_scale.shape[3]
+        if not blocks or cap % blocks:
+            raise _bad(f"{blocks} blocks for a capacity of {cap}")
+        for name, t, shape, dt in (("k", k, (b, layers, heads, cap, d), torch.uint8), ("v", v, (b, layers, heads, d, cap), torch.uint8),
+                                   ("k_scale", k_scale, (b, layers, heads, blocks), torch.float32),
+                                   ("v_scale", v_scale, (b, layers, heads, blocks), torch.float32),
+                                   ("lens", lens, (b,), torch.int32)):
+            if tuple(t.shape) != shape or t.dtype != dt or not t.is_contiguous() or t.device != k.device or not t.is_cuda:
+                raise _bad(f"'{name}' must be a contiguous {dt} CUDA tensor of shape {shape} on k's device, "
+                           f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+        self.k, self.v, self.k_scale, self.v_scale, self.lens = k, v, k_scale, v_scale, lens
+        self.batch, self.layers, self.heads, self.capacity, self.head_dim = b, layers, heads, cap, d
+        self.block = cap // blocks
+        self.device = k.device
+        self.lib = C.load_library()
+        self._c = C.FaKv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), b, layers, heads, d, cap,
+                          self.block)
+        self._ref = ctypes.byref(self._c)
+        self._ws = {}  # workspace bytes of the shapes asked for
+
+    def _check(self, st):
+        if st != C.FA_OK:
+            C.check(self.lib, None, st)
+
+    def _on(self, stream, fn):
+        """Runs fn(raw stream) with the cache's device current and, for a stream given, on it."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return fn(stream.cuda_stream)
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return fn(torch.cuda.current_stream(self.device).cuda_stream)
+        return fn(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def _rows(self, name, t, heads):
+        if t.dim() != 4 or t.shape[0] != self.batch or t.shape[2] != heads or t.shape[3] != self.head_dim:
+            raise _bad(f"'{name}' must be [{self.batch}][tokens][{heads}][{self.head_dim}], got {tuple(t.shape)}")
+        if t.device != self.device:
+            raise _bad(f"'{name}' is on {t.device}, the cache on {self.device}")
+        if t.stride(3) != 1:
+            t = t.contiguous()
+        return t, C.FaRows(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+
+    def _ints(self, name, t):
+        if t is None:
+            return None
+        if t.dtype != torch.int32 or tuple(t.shape) != (self.batch,) or not t.is_contiguous() or t.device != self.device:
+            raise _bad(f"'{name}' must be a contiguous int32 tensor [{self.batch}] on {self.device}")
+        return t.data_ptr()
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, *, count: torch.Tensor | None = None,
+               start: torch.Tensor | None = None, stream=None):
+        """Quantises k, v [batch][tokens][heads][head_dim] (fp32, bf16 or fp16, any strides) into `layer` behind `start`
+        (default: lens). count (int32 [batch]) gives each observation's number of real rows in a padded batch."""
+        if k.dtype not in _DT or v.dtype != k.dtype:
+            raise _bad(f"k and v must share fp32, bf16 or fp16, got {k.dtype} and {v.dtype}")
+        if k.dim() == 4 and v.dim() == 4 and k.shape[1] != v.shape[1]:
+            raise _bad(f"{k.shape[1]} rows of k and {v.shape[1]} of v")
+
+        def call(s):
+            (kt, kr), (vt, vr) = self._rows("k", k, self.heads), self._rows("v", v, self.heads)
+            self._check(self.lib.fa_kv8_append(self._ref, layer, k.shape[1], ctypes.byref(kr), ctypes.byref(vr), _DT[k.dtype],
+                                               self._ints("start", self.lens if start is None else start),
+                                               self._ints("count", count), s))
+        self._on(stream, call)
+
+    def advance(self, n):
+        """lens += n (a number, or a tensor [batch]) after every layer has appended."""
+        self.lens += n
+
+    def attend(self, layer: int, q: torch.Tensor, *, scale: float | None = None, causal: bool = True,
+               prefix: torch.Tensor | None = None, q_lens: torch.Tensor | None = None, lens: torch.Tensor | None = None,
+               max_len: int = 0, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """softmax(scale q K^T + mask) V for q [batch][tokens][q_heads][head_dim] (bf16 or fp16, any strides); scale
+        defaults to head_dim ** -0.5. lens (default: the cache's) counts the cached tokens, the queries' own among
+        them. causal: token i of an observation's q_lens (default: tokens) stands at lens - q_lens + i and sees the
+        keys up to there, and all below prefix; not causal: every key. max_len: an upper bound of lens that the host knows
+        (default: the capacity). Rows of `out` behind q_lens are left as they were (zero in a new tensor)."""
+        if q.dtype not in _DT or q.dim() != 4:
+            raise _bad(f"q must be a bf16 or fp16 tensor of four dimensions, got {q.dtype} {tuple(q.shape)}")
+        b, tokens, q_heads, d = q.shape
+
+        def call(s):
+            qt, qr = self._rows("q", q, q_heads)
+            o = out
+            if o is None:
+                o = (torch.empty if q_lens is None else torch.zeros)((b, tokens, q_heads, d), dtype=q.dtype, device=q.device)
+            elif o.shape != q.shape or o.dtype != q.dtype or o.device != q.device or (o.numel() and o.stride(3) != 1):
+                raise _bad(f"'out' must be like q ({q.dtype} {tuple(q.shape)}) with a contiguous last dimension")
+            orow = C.FaRows(o.data_ptr(), o.stride(0), o.stride(1), o.stride(2))
+            key = (tokens, q_heads, max_len)
+            need = self._ws.get(key)
+            if need is None:
+                n = ctypes.c_size_t()
+                self._check(self.lib.fa_kv8_attention_workspace(self._ref, tokens, q_heads, max_len, ctypes.byref(n)))
+                need = self._ws[key] = n.value
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+            self._check(self.lib.fa_kv8_attention(
+                self._ref, layer, tokens, q_heads, ctypes.byref(qr), _DT[q.dtype], self._ints("lens", self.lens if lens is None else lens),
+                self._ints("q_lens", q_lens), self._ints("prefix", prefix), int(causal), d ** -0.5 if scale is None else scale,
+                max_len, ctypes.byref(orow), ws.data_ptr() if need else None, need, s))
+            return o
+        return self._on(stream, call)
+
+    def read(self, rows: int, *, dtype=torch.bfloat16, lens: torch.Tensor | None = None, stream=None):
+        """(K, V) as values [batch][layers][rows][heads * head_dim], zero at and behind each length."""
+        if dtype not in _DT:
+            raise _bad(f"values are fp32, bf16 or fp16, not {dtype}")
+        if rows < 0:
+            raise _bad(f"rows={rows}")
+
+        def call(s):
+            k, v = (torch.empty(self.batch, self.layers, rows, self.heads * self.head_dim, dtype=dtype, device=self.device)
+                    for _ in range(2))
+            self._check(self.lib.fa_kv8_read(self._ref, self._ints("lens", self.lens if lens is None else lens), rows,
+                                             k.data_ptr(), v.data_ptr(), _DT[dtype], s))
+            return k, v
+        return self._on(stream, call)

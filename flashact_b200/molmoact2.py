@@ -13,7 +13,7 @@ import ctypes
 import torch
 
 from . import _capi as C
-from .pi05 import _DT, _stream_ptr
+from .pi05 import _DT, _stream_ptr, bind_cache
 
 
 class MolmoAct2ActionExpert:
@@ -71,6 +71,11 @@ class MolmoAct2ActionExpert:
             self._check(self.lib.fa_bind_prefix_kv(self.h, B, k.data_ptr(), v.data_ptr(), rows, lens, 0,
                                                    _stream_ptr(stream)))
         self.batch = B
+
+    def bind_context_cache(self, cache, ctx_len=None, stream=None):
+        """Binds the cross-attention context held in a Kv8Cache (heads 8, head_dim 96, the engine's layers): its
+        values go through bind_context as bf16. ctx_len defaults to the cache's lengths, which costs a read back."""
+        bind_cache(self.bind_context, cache, (self.cfg.num_layers, 8, 96), ctx_len, stream)
 
     def sample_actions(self, noise: torch.Tensor, out=None, stream=None, sync=True):
         noise = noise.float().contiguous()

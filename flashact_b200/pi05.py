@@ -22,6 +22,21 @@ def _stream_ptr(stream=None):
     return ctypes.c_void_p(s.cuda_stream)
 
 
+def bind_cache(bind, cache, want, valid_len, stream):
+    """Reads a Kv8Cache of `want` = (layers, heads, head_dim) and hands its values to an engine's bind."""
+    have = (cache.layers, cache.heads, cache.head_dim)
+    if have != want:
+        raise C.FlashActError(C.FA_ERR_INVALID, f"a cache of layers, heads, head_dim {have}: the engine has {want}")
+    if valid_len is None:
+        with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(cache.device)):
+            valid_len = cache.lens.tolist()
+    valid_len = [int(x) for x in valid_len]
+    if len(valid_len) != cache.batch or min(valid_len) < 0 or max(valid_len) > cache.capacity:
+        raise C.FlashActError(C.FA_ERR_INVALID, f"lengths {valid_len} for a cache of {cache.batch} x {cache.capacity} tokens")
+    k, v = cache.read(max(1, max(valid_len)), stream=stream)
+    bind(k, v, valid_len, stream=stream)
+
+
 class Pi05ActionExpert:
     """Owns one fa_handle on one device. Weights: dict with the keys of
     flashact_b200._capi.PI05_WEIGHT_FIELDS, [out][in] row-major, stacked over layers."""
@@ -98,6 +113,12 @@ class Pi05ActionExpert:
             self._check(self.lib.fa_bind_prefix_kv(self.h, B, k.data_ptr(), v.data_ptr(), rows, vl, lay,
                                                    _stream_ptr(stream)))
         self.batch = B
+
+    def bind_prefix_cache(self, cache, valid_len=None, stream=None):
+        """Binds the prefix held in a Kv8Cache (heads 1, head_dim 256, the engine's layers; K in the split-half RoPE
+        order): its values go through bind_prefix_kv as bf16. valid_len (host numbers, as there)
+        defaults to the cache's lengths, which costs a read back."""
+        bind_cache(self.bind_prefix_kv, cache, (self.cfg.num_layers, 1, 256), valid_len, stream)
 
     def sample_actions(self, noise: torch.Tensor, out: torch.Tensor | None = None, stream=None,
                        sync: bool = True) -> torch.Tensor:

@@ -1,5 +1,5 @@
 """On-device FP8 / NVFP4 weight quantisation (fa_quantize_fp8_rows / fa_quantize_nvfp4 in
-include/flashact.h): the codes and scales Pi05ActionExpert(wfmt="fp8" | "nvfp4") takes, computed
+include/flashact.h) and the product with NVFP4 weights (fa_nvfp4_linear): the codes and scales Pi05ActionExpert(wfmt="fp8" | "nvfp4") takes, computed
 on the GPU from bf16 / fp16 / fp32 weights. The reference quantises on the host inside
 HybridPi05._pack_weights (src/pi05/hybrid_model.py:105-110). No CPU fallback."""
 from __future__ import annotations
@@ -56,3 +56,43 @@ def quantize_nvfp4(w: torch.Tensor):
                                           ctypes.c_void_p(packed.data_ptr()), ctypes.c_void_p(bscale.data_ptr()),
                                           ctypes.c_void_p(tscale.data_ptr()), _stream_ptr()))
     return packed, bscale, tscale
+
+
+def nvfp4_linear(x: torch.Tensor, packed: torch.Tensor, block_scale: torch.Tensor, tensor_scale: torch.Tensor, *,
+                 bias: torch.Tensor | None = None, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """x W^T * tensor_scale (+ bias) for x [..., K] (bf16 or fp16) of up to 16 rows and one layer's matrix as
+    quantize_nvfp4 gives it: packed uint8 [N, K/2], block_scale uint8 [N, K/16], tensor_scale fp32 of one element;
+    bias fp32 [N]. Returns [..., N] in x's type."""
+    lib = C.load_library()
+    if x.dim() < 1 or x.dtype not in _DT or not x.is_cuda:
+        raise C.FlashActError(C.FA_ERR_INVALID, "x must be a CUDA tensor [..., K]")
+    K, dev = x.shape[-1], x.device
+    N = packed.shape[0] if packed.dim() == 2 else 0
+    for name, t, shape, dt in (("packed", packed, (N, K // 2), torch.uint8), ("block_scale", block_scale, (N, K // 16), torch.uint8),
+                               ("tensor_scale", tensor_scale, None, torch.float32), ("bias", bias, (N,), torch.float32)):
+        if t is None and name == "bias":
+            continue
+        if (t.numel() != 1 if shape is None else t.shape != shape) or t.dtype != dt or t.device != dev or not t.is_contiguous():
+            raise C.FlashActError(C.FA_ERR_INVALID, f"'{name}' must be a contiguous {dt} tensor {shape or '(one element)'} on "
+                                                    f"{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    shape = (*x.shape[:-1], N)
+    if out is not None and (out.shape != shape or out.dtype != x.dtype or out.device != dev or not out.is_contiguous()):
+        raise C.FlashActError(C.FA_ERR_INVALID, f"'out' must be a contiguous {x.dtype} tensor {tuple(shape)} on {dev}")
+
+    def call(s):
+        xc = x.contiguous()
+        if xc.data_ptr() % 16:
+            xc = xc.clone()
+        y = torch.empty(shape, dtype=x.dtype, device=dev) if out is None else out
+        _check(lib, lib.fa_nvfp4_linear(xc.data_ptr(), _DT[x.dtype], xc.numel() // K if K else 0, K, K, packed.data_ptr(),
+                                        block_scale.data_ptr(), tensor_scale.data_ptr(),
+                                        None if bias is None else bias.data_ptr(), N, y.data_ptr(), N, s))
+        return y
+
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return call(stream.cuda_stream)
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return call(torch.cuda.current_stream(dev).cuda_stream)
+    return call(torch.cuda.current_stream(dev).cuda_stream)

@@ -134,6 +134,74 @@ FA_API fa_status fa_quantize_fp8_rows(const void* w, fa_dtype dtype, int L, int 
 FA_API fa_status fa_quantize_nvfp4(const void* w, fa_dtype dtype, int L, int rows, int K, unsigned char* packed,
                                    unsigned char* block_scale, float* tensor_scale, fa_stream stream);
 
+/* y = x W^T * tensor_scale (+ bias), W [N][K] in NVFP4 as fa_quantize_nvfp4 writes one layer of it
+ * (packed [N][K/2], block_scale [N][K/16], tensor_scale one fp32): the codes are read as they are, 9/16 of a
+ * byte a weight, and their products with the block scales are exact in x's type. x [M][K] (row stride ldx,
+ * a multiple of 8) and y [M][N] (row stride ldy) in `dtype` (bf16 or fp16), bias fp32 [N] or NULL; M <= 16
+ * (0: nothing is done), K a multiple of 16. Sums are fp32, rounded once. Device memory of the current
+ * device, x 16-byte and packed 8-byte aligned; asynchronous on `stream`, no workspace, results do not
+ * depend on timing. Errors are read with fa_last_error(NULL). */
+FA_API fa_status fa_nvfp4_linear(const void* x, fa_dtype dtype, int M, int K, long long ldx, const unsigned char* packed,
+                                 const unsigned char* block_scale, const float* tensor_scale, const float* bias, int N,
+                                 void* y, long long ldy, fa_stream stream);
+
+/* ---- 8-bit KV cache ----
+ * The keys and values of a prefix in E4M3 with one fp32 scale for each block of `block` tokens and head: half the
+ * bytes of the bf16 prefix. value = code x scale of its block. K is kept token by token, V transposed (both
+ * then feed the attention's products along contiguous bytes).
+ *   k       [batch][layers][heads][capacity][head_dim] codes
+ *   v       [batch][layers][heads][head_dim][capacity] codes
+ *   k_scale, v_scale [batch][layers][heads][capacity / block]
+ * head_dim 64, 96, 128 or 256; block 16, 32, 64 or 128; capacity a multiple of block. k and v 16-byte aligned.
+ * The caller owns the memory and the lengths; no call changes a length. The calls keep nothing between them
+ * and take device memory of the current device, asynchronous on `stream`; lengths are read on the device, so
+ * that a captured call follows them. Errors are read with fa_last_error(NULL). */
+typedef struct fa_kv8 {
+  unsigned char *k, *v;
+  float *k_scale, *v_scale;
+  int batch, layers, heads, head_dim, capacity, block;
+} fa_kv8;
+
+/* Rows [batch][token][head][head_dim] with strides in elements; head_dim is contiguous. */
+typedef struct fa_rows {
+  void* ptr;
+  long long batch, token, head;
+} fa_rows;
+
+/* Quantises `rows` new tokens of each observation into layer `layer` at positions start[b]...: scale = the
+ * smallest power of two s >= 2^-96 with amax <= 448 s over the new rows of a block and head, no smaller than
+ * the block's scale where the block already holds tokens before start[b]; code = E4M3(x / s), nearest
+ * even. Tokens that are already in such a block keep their values on the larger scale (exact but for codes that
+ * become subnormal). Infinities saturate, NaN is stored as 0 and neither sets the scale: the cache never holds
+ * a NaN code. k, v in `dtype` (f32, bf16, f16); start, count device int32 [batch]. count (NULL: rows) gives
+ * each observation's number of new rows, 0..rows; what would lie behind the capacity is dropped. Appending the same
+ * rows at the same start again changes nothing. */
+FA_API fa_status fa_kv8_append(const fa_kv8* c, int layer, int rows, const fa_rows* k, const fa_rows* v,
+                               fa_dtype dtype, const int* start, const int* count, fa_stream stream);
+
+/* The values of the cache as [batch][layers][rows][heads * head_dim] in `dtype` (f32, bf16: exact where scales are
+ * powers of two; f16), k and v 16-byte aligned: the layout fa_bind_prefix_kv takes. lens device int32
+ * [batch]; rows at and behind lens[b] are zero. */
+FA_API fa_status fa_kv8_read(const fa_kv8* c, const int* lens, int rows, void* k, void* v, fa_dtype dtype,
+                             fa_stream stream);
+
+/* Attention of `tokens` query tokens over layer `layer`: out = softmax(scale q K^T + mask) V in fp32, rounded once to
+ * the queries' type (`dtype`: bf16 or f16). q and out are [batch][tokens][q_heads][head_dim] rows; query head
+ * i reads key head i / (q_heads / heads). lens, q_lens, prefix: device int32 [batch]. lens[b] tokens
+ * of observation b are in the cache, the queries' own included where they attend to themselves; q_lens[b] (NULL:
+ * tokens) of its query tokens are real: the output rows of the others are left as they were. Query token i
+ * stands at position lens[b] - q_lens[b] + i. causal: it sees the keys up to its position, and all below prefix[b] (NULL: 0); not
+ * causal: all lens[b]. A query that sees no key gets zeros. max_len is an upper bound of lens known to the host
+ * (0: capacity); lengths above it count as it. The work is split by max_len, and the splits are joined in a fixed
+ * order: results do not depend on timing. workspace: fa_kv8_attention_workspace bytes, 16-byte aligned,
+ * nothing kept in it between calls; calls that overlap on the GPU need one each. Codes behind lens[b]
+ * may hold anything; a NaN code before it makes the result of its head NaN, masked or not. */
+FA_API fa_status fa_kv8_attention_workspace(const fa_kv8* c, int tokens, int q_heads, int max_len, size_t* bytes);
+FA_API fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, int q_heads, const fa_rows* q, fa_dtype dtype,
+                                  const int* lens, const int* q_lens, const int* prefix, int causal, float scale,
+                                  int max_len, const fa_rows* out, void* workspace, size_t workspace_bytes,
+                                  fa_stream stream);
+
 /* MolmoAct2 action-expert weights (benchmarks/molmoact2/eval_numerics.py:77-100 names), stacked
  * over the L blocks, [out][in] row-major: self_attn.qkv, self_attn.out_proj, cross_attn.q_proj,
  * cross_attn.out_proj, mlp.{gate,up,down}_proj (+ biases), action_embed, final_layer.linear. */
