@@ -12,9 +12,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIB_DIR, "libflashact.so")
 SOURCES = ["pi05_kernel.cu", "ma2_kernel.cu", "host_pi05.cu", "host_ma2.cu", "host_quant.cu", "host_nvfp4.cu",
-           "host_kv8.cu", "host_kv8_attn.cu", "kv8_attn_few.cu"]
+           "host_kv8.cu", "host_kv8_attn.cu", "kv8_attn_few.cu", "kv8_attn_rows.cu"]
 DEPS = SOURCES + ["fa_pi05.cuh", "fa_ma2.cuh", "fa_ptx.cuh", "fa_engine.cuh", "fa_engine_types.cuh", "host_common.cuh",
-                  "fa_kv8.cuh", "kv8_attn.cuh"]
+                  "fa_kv8.cuh", "kv8_attn.cuh", "kv8_tc.cuh"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
          "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr"]

@@ -12,21 +12,27 @@ namespace kv8 {
 constexpr float kE4M3Max = 448.0f;
 constexpr int kMinExp = -96;  // smallest block scale 2^-96: its reciprocal and 448 / 2^-96 stay finite
 
-// Two E4M3 codes -> two f16 values, exact (every E4M3 value is an f16 value).
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t two) {
+// Codes 0, 1 (lo) and 2, 3 (hi) of a word -> two f16 values each, exact (every E4M3 value is an f16 value).
+__device__ __forceinline__ uint32_t e4m3_lo_f16x2(uint32_t four) {
   uint32_t r;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two));
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(four));
   return r;
 }
-__device__ __forceinline__ uint32_t e4m3x2_f16x2_hi(uint32_t four) {
+__device__ __forceinline__ uint32_t e4m3_hi_f16x2(uint32_t four) {
   uint32_t r;
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(four));
+  return r;
+}
+// An 8x8 matrix of 16-bit values, two neighbours of row (lane / 4) in a lane's word, turned around.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 
 // D(16x8, f32) += A(16x16, f16) B(16x8, f16).
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -99,6 +105,8 @@ static inline fa_status kv8_check(const fa_kv8* c) {
   if (!c) return fail(nullptr, FA_ERR_INVALID, "null cache");
   if (c->batch < 1 || c->batch > 65535 || c->layers < 1 || c->heads < 1 || c->heads > 65535)
     return fail(nullptr, FA_ERR_INVALID, "cache of batch=%d layers=%d heads=%d", c->batch, c->layers, c->heads);
+  if ((long long)c->batch * c->layers > 0x7fffffffLL / c->heads)
+    return fail(nullptr, FA_ERR_INVALID, "batch x layers x heads is over 2^31 - 1");
   if (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128 && c->head_dim != 256)
     return fail(nullptr, FA_ERR_UNSUPPORTED, "head_dim=%d is not 64, 96, 128 or 256", c->head_dim);
   if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128)

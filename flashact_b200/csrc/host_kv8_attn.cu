@@ -1,35 +1,86 @@
-// fa_kv8_attention: checks, the split of the key axis, and the choice of kernel.
-#include "kv8_attn.cuh"
+// fa_kv8_attention: checks, the split of the key axis, the choice of kernel, and the merge of the splits.
+#include "kv8_tc.cuh"
 
 namespace {
 
 using namespace fa::kv8;
 
 struct Plan {
-  int tiles, nsplit, split_chunks;
+  int rows, tiles, nsplit, cluster, split_chunks;
   size_t part_bytes, ml_bytes;
 };
 
-// Few query rows (kv8_attn_few.cu): 16 rows a tile, CTAs of four warps that take 64-key chunks in turn, two CTAs
-// on an SM. The split count is the one with the least rounds of chunks on the busiest SM slot, each wave
-// of CTAs paying about two rounds for its start and a merge about three.
-Plan plan_few(const fa_kv8* c, int tokens, int q_heads, int max_len, int sms) {
+// One warp per query row: o = sum_s 2^(m_s - m) part_s / sum_s 2^(m_s - m) l_s over the splits that the
+// row's tile has, in split order (the result does not depend on which split ended first).
+template <int D>
+__global__ void merge_kernel(const AttnArgs a) {
+  const int lane = threadIdx.x & 31, h = blockIdx.y, b = blockIdx.z, R = a.rows;
+  const int row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  wait_for_primary();
+  const int n = a.mask.len(b), nq = a.mask.q_len(b), pre = a.mask.prefix ? a.mask.prefix[b] : 0;
+  if (row >= nq * a.group) return;
+  const int tile = row / R, r = row % R, last = min(tile * R + R, nq * a.group) - 1;
+  const int top = a.mask.limit(n, nq, pre, token_of(a, last)), lim = a.mask.limit(n, nq, pre, token_of(a, row));
+  const int chunks = (top + TILE - 1) / TILE;
+  const int used = max(1, (chunks + a.split_chunks - 1) / a.split_chunks);
+  const size_t slot = (((size_t)b * a.heads + h) * a.tiles + tile) * a.nsplit;
+  float m = -INFINITY, l = 0.f;
+  for (int s = lane; s < used; s += 32) m = fmaxf(m, a.ml[(slot + s) * R + r].x);
+  m = warp_max(m);
+  const float base = m == -INFINITY ? 0.f : m;
+  float acc[D / 32] = {};
+#pragma unroll 4
+  for (int s = 0; s < used; ++s) {
+    const float2 x = a.ml[(slot + s) * R + r];
+    const float f = exp2_approx(x.x - base);
+    l += x.y * f;
+    const float* p = a.part + ((slot + s) * R + r) * D + lane;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] += f * p[i * 32];
+  }
+  const float norm = 1.0f / l;
+  const long long oo = row_at(a, b, h, row, a.ob, a.ot, a.oh) + lane;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) store16(a.out, oo + i * 32, lim > 0 ? acc[i] * norm : 0.f, a.half);
+}
+
+// 3D byte map [outer][rows][inner] with boxes {128, box_rows, 1}, 128-byte swizzle; what lies outside reads as zero.
+fa_status byte_map(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t outer, uint32_t box_rows) {
+  auto enc = get_encode();
+  if (!enc) return fail(nullptr, FA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[3] = {inner, rows, outer};
+  cuuint64_t strides[2] = {inner, inner * rows};
+  cuuint32_t box[3] = {128, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(nullptr, FA_ERR_CUDA, "cuTensorMapEncodeTiled (cache) failed (%d)", (int)r);
+  return FA_OK;
+}
+
+// The kernel and the splits of whole 128-key tiles.
+Plan make_plan(const fa_kv8* c, int tokens, int q_heads, int max_len, int sms) {
   Plan p;
-  const int rows = 16, warps = 4, slots = 2 * sms;
-  p.tiles = (int)(((long long)tokens * (q_heads / c->heads) + rows - 1) / rows);
-  const int chunks = std::max(1, (max_len + 63) / 64);
+  const long long all = (long long)tokens * (q_heads / c->heads);
+  p.rows = all <= 8 ? 8 : all <= 16 ? 16 : 128;
+  p.tiles = (int)((all + p.rows - 1) / p.rows);
+  const int chunks = std::max(1, (max_len + 127) / 128), slots = (p.rows == 128 ? 1 : 2) * sms;
   const long long base = (long long)c->batch * c->heads * p.tiles;
+  const double mb = 256e-6 * c->head_dim;  // a tile's bytes, in MB
   double best = 1e300;
   p.nsplit = 1;
-  for (int n = 1; n <= 64 && n <= (chunks + warps - 1) / warps; ++n) {
-    const int each = (chunks + n - 1) / n, rounds = (each + warps - 1) / warps;
-    const double waves = (double)((base * n + slots - 1) / slots);
-    const double cost = waves * (rounds + 2) + (n > 1 ? 3 + 0.05 * n : 0);
+  for (int n = 1; n <= 64 && n <= chunks; ++n) {
+    const int each = (chunks + n - 1) / n;
+    const double ctas = (double)base * n, waves = std::ceil(ctas / slots);
+    const double round = std::max(0.5, std::min(ctas, (double)slots) * mb / 6.5);
+    const double cost = waves * (3 + each * round) + (n > 8 ? 2.5 + 0.1 * n : n > 1 ? 1 : 0);
     if (cost < best) best = cost, p.nsplit = n;
   }
   p.split_chunks = (chunks + p.nsplit - 1) / p.nsplit;
   p.nsplit = (chunks + p.split_chunks - 1) / p.split_chunks;
-  const size_t slot = p.nsplit > 1 ? (size_t)base * p.nsplit * rows : 0;
+  p.cluster = p.nsplit > 1 && p.nsplit <= 8;
+  const size_t slot = p.nsplit > 1 && !p.cluster ? (size_t)base * p.nsplit * p.rows : 0;
   p.part_bytes = slot * c->head_dim * sizeof(float);
   p.ml_bytes = slot * sizeof(float2);
   return p;
@@ -61,7 +112,7 @@ extern "C" fa_status fa_kv8_attention_workspace(const fa_kv8* c, int tokens, int
   fa_status st = attn_check(c, tokens, q_heads, max_len);
   if (st != FA_OK) return st;
   if (!bytes) return fail(nullptr, FA_ERR_INVALID, "null bytes");
-  const Plan p = plan_few(c, std::max(1, tokens), q_heads, max_len ? max_len : c->capacity, sm_count());
+  const Plan p = make_plan(c, std::max(1, tokens), q_heads, max_len ? max_len : c->capacity, sm_count());
   *bytes = p.part_bytes + p.ml_bytes;
   return FA_OK;
 }
@@ -82,7 +133,7 @@ extern "C" fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, in
     return fail(nullptr, FA_ERR_INVALID, "queries and output must be aligned to their type");
   if (tokens == 0) return FA_OK;
   const int top = max_len ? max_len : c->capacity;
-  const Plan p = plan_few(c, tokens, q_heads, top, sm_count());
+  const Plan p = make_plan(c, tokens, q_heads, top, sm_count());
   if (workspace_bytes < p.part_bytes + p.ml_bytes)
     return fail(nullptr, FA_ERR_INVALID, "workspace of %zu bytes, %zu are needed", workspace_bytes, p.part_bytes + p.ml_bytes);
   if (p.part_bytes && reinterpret_cast<uintptr_t>(workspace) % 16)
@@ -98,11 +149,36 @@ extern "C" fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, in
   a.qb = q->batch, a.qt = q->token, a.qh = q->head;
   a.ob = out->batch, a.ot = out->token, a.oh = out->head;
   a.mask = Mask{lens, q_lens, prefix, causal != 0, tokens, top};
-  a.layers = c->layers, a.layer = layer, a.heads = c->heads, a.group = q_heads / c->heads, a.cap = c->capacity;
-  a.block = c->block, a.half = dtype == FA_DT_F16;
+  a.layers = c->layers, a.layer = layer, a.heads = c->heads, a.group = q_heads / c->heads, a.dim = c->head_dim, a.cap = c->capacity;
+  a.blocks = c->capacity / c->block, a.block_log2 = __builtin_ctz(c->block), a.half = dtype == FA_DT_F16;
+  a.q_wide = reinterpret_cast<uintptr_t>(q->ptr) % 16 == 0 && q->batch % 8 == 0 && q->token % 8 == 0 && q->head % 8 == 0;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.nsplit = p.nsplit, a.split_chunks = p.split_chunks, a.tiles = p.tiles;
+  a.group_mul = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
+  a.nsplit = p.nsplit, a.cluster = p.cluster, a.split_chunks = p.split_chunks, a.rows = p.rows, a.tiles = p.tiles;
   a.part = reinterpret_cast<float*>(workspace);
   a.ml = reinterpret_cast<float2*>(reinterpret_cast<char*>(workspace) + p.part_bytes);
-  return kv8_launch_few(a, c->head_dim, c->batch, reinterpret_cast<cudaStream_t>(stream));
+  CUtensorMap km, vm;
+  const uint64_t outer = (uint64_t)c->batch * c->layers * c->heads;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if ((st = byte_map(&km, c->k, c->head_dim, c->capacity, outer, TILE)) != FA_OK) return st;
+  if ((st = byte_map(&vm, c->v, c->capacity, c->head_dim, outer, c->head_dim <= 128 ? 128 : 256)) != FA_OK) return st;
+  st = p.rows == 128 ? kv8_launch_rows(a, c->batch, km, vm, s) : kv8_launch_few(a, c->batch, km, vm, s);
+  if (st != FA_OK || p.nsplit == 1 || p.cluster) return st;
+  // The merge is set up while the attention runs (programmatic dependent launch): its own launch costs nothing then.
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((tokens * a.group + 3) / 4, c->heads, c->batch);
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  switch (c->head_dim) {
+    case 64: FA_CUDA(nullptr, cudaLaunchKernelEx(&cfg, merge_kernel<64>, a)); break;
+    case 96: FA_CUDA(nullptr, cudaLaunchKernelEx(&cfg, merge_kernel<96>, a)); break;
+    case 128: FA_CUDA(nullptr, cudaLaunchKernelEx(&cfg, merge_kernel<128>, a)); break;
+    default: FA_CUDA(nullptr, cudaLaunchKernelEx(&cfg, merge_kernel<256>, a)); break;
+  }
+  return FA_OK;
 }

@@ -12,38 +12,48 @@ struct AttnArgs {
   void* out;
   long long qb, qt, qh, ob, ot, oh;  // element strides: batch, token, head
   Mask mask;
-  int layers, layer, heads, group, cap, block, half;  // half: fp16 queries (else bf16)
+  int layers, layer, heads, group, dim, cap, blocks, block_log2, half, q_wide;  // half: fp16 queries (else bf16); q_wide: their rows are 16-byte aligned
   float scale_log2;  // score scale * log2(e)
-  int nsplit, split_chunks;  // splits of the key axis; chunks of one split
+  uint32_t group_mul;  // ceil(2^32 / group): token of a row without a division
+  // Splits of the key axis, joined by the cluster that they are (at most 8), or by the merge kernel. With a cluster
+  // each takes an equal share of the observation's own tiles, else tiles [split * split_chunks, + split_chunks).
+  int nsplit, cluster, split_chunks;
+  int rows;                  // rows of a tile
   int tiles;                 // row tiles of a (observation, key head)
   float* part;               // [slot][rows of a tile][D] unnormalised sums, slot = ((b, h), tile, split)
   float2* ml;                // [slot][rows of a tile]: max (log2 units) and sum
 };
 
-// A power of two near |x|'s largest value, its exponent cleared of extremes: x * 2^-e is in [1, 2).
-__device__ __forceinline__ float row_pow2(float amax) {
-  const int x = (__float_as_int(amax) >> 23) - 127;
-  return (amax > 0.f && x < 127 && x > -100) ? __int_as_float((x + 127) << 23) : 1.0f;
+// row / group; rows are below 2^24 + 128, so the product is at most one too high.
+__device__ __forceinline__ int token_of(const AttnArgs& a, int row) {
+  if (a.group == 1) return row;
+  const int t = (int)__umulhi((uint32_t)row, a.group_mul);
+  return t - (t * a.group > row);
 }
-__device__ __forceinline__ float load16(const void* p, long long i, int half) {
-  return half ? __half2float(reinterpret_cast<const __half*>(p)[i]) : __bfloat162float(reinterpret_cast<const bf16*>(p)[i]);
+// First element of a row (token, head) of the queries or of the output.
+__device__ __forceinline__ long long row_at(const AttnArgs& a, int b, int h, int row, long long sb, long long st, long long sh) {
+  const int t = token_of(a, row);
+  return b * sb + t * st + (h * a.group + row - t * a.group) * sh;
 }
-// Two consecutive 16-bit outputs: one store where the row is 4-byte aligned.
-__device__ __forceinline__ void store16x2(void* p, long long i, float x, float y, int half) {
-  const uint32_t hv = pack_f16x2(x, y);
-  const __nv_bfloat162 bv = __floats2bfloat162_rn(x, y);
-  const uint32_t v = half ? hv : *reinterpret_cast<const uint32_t*>(&bv);
-  uint16_t* q = reinterpret_cast<uint16_t*>(p) + i;
-  if ((reinterpret_cast<uintptr_t>(q) & 3) == 0) {
-    *reinterpret_cast<uint32_t*>(q) = v;
-  } else {
-    q[0] = (uint16_t)v;
-    q[1] = (uint16_t)(v >> 16);
-  }
+
+// A row of queries is multiplied by 2^(7 - x), x the exponent of its largest magnitude, which brings that to [128, 256); x = 0
+// for a row of zeros or of numbers below 2^-100. `back` undoes it; it is NaN for a row with an infinity, whose scores and
+// outputs then are NaN.
+__device__ __forceinline__ float row_factor(float amax, float& back) {
+  int x = (__float_as_int(amax) >> 23) - 127;
+  const bool inf = x > 127;
+  x = x > -100 && !inf ? x : 0;
+  back = inf ? __int_as_float(0x7fffffff) : __int_as_float((x - 7 + 127) << 23);
+  return __int_as_float((7 - x + 127) << 23);
+}
+__device__ __forceinline__ void store16(void* p, long long i, float x, int half) {
+  if (half) reinterpret_cast<__half*>(p)[i] = __float2half(x);
+  else reinterpret_cast<bf16*>(p)[i] = __float2bfloat16(x);
 }
 
 }  // namespace kv8
 }  // namespace fa
 
-// Launchers (kv8_attn_few.cu). `dim` is the head dimension.
-fa_status kv8_launch_few(const fa::kv8::AttnArgs& a, int dim, int batch, cudaStream_t s);
+// The kernels: up to 16 query rows of a key head (kv8_attn_few.cu), and 128 at a time (kv8_attn_rows.cu).
+fa_status kv8_launch_few(const fa::kv8::AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s);
+fa_status kv8_launch_rows(const fa::kv8::AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s);

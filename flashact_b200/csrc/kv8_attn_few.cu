@@ -1,374 +1,437 @@
-// Attention over the 8-bit cache for few query rows of a key head (one token of grouped heads),
-// bound by the cache's bytes; and the merge of the splits.
+// Attention over the 8-bit cache for up to 16 query rows of a key head, on the tensor cores' 8-bit kind.
 //
-// o = sum_j p_j vs_j V_j / sum_j p_j with p_j = 2^(s_j - max s), s_j = log2(e) scale ks_j (q . K_j):
-// the codes K_j, V_j go to the matrix instruction as f16 (exact), the block scales ks and vs multiply
-// the scores and the probabilities, which a thread holds for 16 consecutive keys of a 64-key chunk
-// and so, with blocks of 16 or more, one factor each. q is scaled per row by a power of two into f16
-// (exact: f16 has more bits than bf16, and what falls below 2^-24 of the row's largest element is
-// below the scores' own rounding).
+// o = sum_j p_j vs_j V_j / sum_j p_j with p_j = 2^(s_j - max s), s_j = log2(e) scale ks_j (q . K_j). The cache's codes
+// are the 128-row operand of both products as TMA brings them, S^T = K Q^T (128 keys by the query rows) and O^T = V^T P^T (128
+// dims by the query rows), and nothing of the cache is converted. The other operand has more bits than eight: it is given in parts, each the
+// 8-bit rounding of what the parts before it left over, scaled up, and each part has its own columns of the product, so
+// that a part costs no further pass over the cache:
+//   queries  E4M3 parts in units 1, 1/16 (1/256 for fp16), a row scaled by a power of two to [128, 256): bf16 rows are
+//            exact down to 2^-21 of their largest element, fp16 rows to 2^-25;
+//   P        E5M2 parts in units 1, 1/8, 1/64 (1/512 for fp16) of p * 2^12 * vs / (the split's largest vs) rounded to f16:
+//            2^-10 of each p (fp16: 2^-11), its smallest 2^-36: E5M2's range keeps what thousands of faint keys add up to
+//            next to one loud key.
+// The block scales ks, vs multiply scores and probabilities: a thread of the softmax is a key, and has one of each.
 //
-// Each warp works alone on every fourth 64-key chunk of the CTA's split, with its own running
-// maximum and sum. The matrix instruction's operand order along d and along the keys is free as long as
-// both operands share it: lane (g, t) owns bytes [16 t, 16 t + 16) of a row, so K and V are fetched in
-// 16-byte pieces by the lane that uses them, through a ring of shared memory that no other lane
-// reads (cp.async groups, no barrier in the loop).
-#include "kv8_attn.cuh"
+// One CTA takes R query rows of a (observation, key head) and a split of the keys in tiles of 128: warp 0 keeps a ring
+// of K and V tiles full, warp 1 issues the products (scores of tile i + 1 before P V of tile i), warps 2..5 turn scores into
+// probabilities. The running maximum moves only where it grew by more than 2^3, the only case that touches O^T.
+#include "kv8_tc.cuh"
 
 namespace {
 
 using namespace fa;
 using namespace fa::kv8;
 
-constexpr int WARPS = 4, DEPTH = 6, CHUNK = 64, ROWS = 16;
-constexpr float kPOff = 12.0f;  // probabilities are held as p * 2^12 in f16: down to 2^-36 of the largest
+constexpr int THREADS = 192;
+constexpr float kPTop = 4096.0f;  // p = 1; with a maximum that lags by up to kLag, 2^15 (E5M2 ends at 57344)
+constexpr float kLag = 3.0f;
 
-template <int D>
-struct Few {
-  static constexpr int NK = (D + 63) / 64;      // K pieces of 64 dims (the last may be 32)
-  static constexpr int NV = (D + 63) / 64;      // V pieces of 64 dims
-  static constexpr int NSUB = NK + NV;
-  static constexpr int KSTEPS = D / 16;
-  static constexpr int SLOT = 4096;             // 8 pieces x 32 lanes x 16 bytes
-  static constexpr int RING = WARPS * DEPTH * SLOT;
-  static constexpr int MERGE = WARPS * ROWS * D * 4;
-  static constexpr int QF = KSTEPS * 32 * 16;
-  static constexpr int BODY = RING > MERGE ? RING : MERGE;
-  static constexpr int SMEM = QF + BODY + 1024;
+__device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// R query rows; QP, PP parts of the queries and of P; MT tiles of 128 dims.
+template <int R_, bool HALF, int MT_>
+struct Cfg {
+  static constexpr int R = R_, MT = MT_;
+  static constexpr int QP = HALF ? 3 : 2, PP = HALF ? 4 : 3;
+  static constexpr int NS = align_up(R * QP, 16), NP = align_up(R * PP, 16);  // columns of S^T and of O^T
+  static constexpr int SLOT = MT * 16384;                                     // one K or V tile
+  static constexpr int COLS = 2 * NS + MT * NP <= 128 ? 128 : 2 * NS + MT * NP <= 256 ? 256 : 512;
+  static constexpr int QBYTES = MT * NS * 128, PBYTES = NP * 128;             // PBYTES: one of two buffers
+  static constexpr int STATE = 2048;                                          // barriers and row state
+  static constexpr int REST = 1024 + QBYTES + 2 * PBYTES + STATE;             // 1024: alignment of the ring
+  // Two CTAs on an SM where each still has three slots, so that one starts while the other works.
+  static constexpr int CTAS = COLS <= 256 && (113 * 1024 - REST) / SLOT >= 3 ? 2 : 1;
+  static constexpr int SLOTS = ((CTAS == 2 ? 113 : 227) * 1024 - REST) / SLOT;
+  static constexpr int SMEM = REST + SLOTS * SLOT;
+  static_assert(SLOTS >= 3 && SLOTS <= 16 && R % 8 == 0 && R <= 16 && 2 * NS + MT * NP <= 512, "shared or tensor memory");
+  static_assert(SLOTS * 16 + 128 <= 480 && 512 + R * 8 + R * 16 + 16 + 32 + R * 8 <= STATE && R * MT * 512 <= SLOTS * SLOT, "state");
 };
 
-template <int D>
-__global__ void __launch_bounds__(WARPS * 32) few_kernel(const AttnArgs a) {
-  using F = Few<D>;
-  extern __shared__ __align__(16) unsigned char smem[];
-  uint4* qf = reinterpret_cast<uint4*>(smem);
-  unsigned char* body = smem + F::QF;
-  float* rowscale = reinterpret_cast<float*>(smem + F::QF + F::BODY);  // [16]
-  int* rowlim = reinterpret_cast<int*>(rowscale + ROWS);               // [16]
-  float* red = reinterpret_cast<float*>(rowlim + ROWS);                // [WARPS]
-  float2* wml = reinterpret_cast<float2*>(red + WARPS);                // [WARPS][16]
+template <int R, bool HALF, int MT>
+__global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
+    few_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using C = Cfg<R, HALF, MT>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  unsigned char* ring = smem;
+  unsigned char* qs = smem + C::SLOTS * C::SLOT;  // [MT][NS][128]
+  unsigned char* ps = qs + C::QBYTES;             // [2][NP][128]
+  unsigned char* state = ps + 2 * C::PBYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(state);  // [SLOTS] tile has landed
+  uint64_t* empty = full + C::SLOTS;                    // [SLOTS] its products are done
+  uint64_t* sfull = empty + C::SLOTS;                   // [2] scores are in tensor memory
+  uint64_t* sfree = sfull + 2;                          // [2] and have been read
+  uint64_t* pfull = sfree + 2;                          // [2] probabilities are in shared memory
+  uint64_t* pvdone = pfull + 2;                         // [2] and their product is done
+  uint64_t* seen = pvdone + 2;                          // [2] the four warps' maxima are in wmax
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(seen + 2);
+  volatile int* err = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  uint64_t* maxes = reinterpret_cast<uint64_t*>(state + 480);  // the four warps' maxima are in wmax
+  float* rowscale = reinterpret_cast<float*>(state + 512);     // [R]
+  int* rowlim = reinterpret_cast<int*>(rowscale + R);          // [R]
+  float* wmax = reinterpret_cast<float*>(rowlim + R);          // [4][R]
+  float* red = wmax + 4 * R;                                   // [4]
+  int* flags = reinterpret_cast<int*>(red + 4);                // [2][4] a warp of the softmax saw a larger maximum
+  float2* mls = reinterpret_cast<float2*>(flags + 8);          // [R] maximum and sum of the split, for the cluster
+  float* osum = reinterpret_cast<float*>(ring);                // [R][PITCH] and its sums, once the ring is done
+  constexpr int PITCH = MT * 128;
 
-  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int tid = threadIdx.x, w = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int split = blockIdx.x % a.nsplit, tile = blockIdx.x / a.nsplit, h = blockIdx.y, b = blockIdx.z;
-  const int n = a.mask.len(b), nq = a.mask.q_len(b), pre = a.mask.prefix ? a.mask.prefix[b] : 0;
-  const int row0 = tile * ROWS, nrows = min(ROWS, nq * a.group - row0);
-  if (nrows <= 0) return;
-  // limits grow with the token: the tile's last row sees the most
-  const int top = a.mask.limit(n, nq, pre, (row0 + nrows - 1) / a.group);
-  const int low = a.mask.limit(n, nq, pre, row0 / a.group);
-  const int chunks = (top + CHUNK - 1) / CHUNK;
-  const int c0 = split * a.split_chunks, c1 = min(chunks, c0 + a.split_chunks);
-  if (c0 >= c1 && split > 0) return;  // split 0 writes the empty rows
-
+  const int row0 = tile * R;
   const size_t hd = ((size_t)b * a.layers + a.layer) * a.heads + h;
-  const unsigned char* kp = a.k + hd * a.cap * D;
-  const unsigned char* vp = a.v + hd * a.cap * D;
-  const float *ks = a.ks + hd * (a.cap / a.block), *vs = a.vs + hd * (a.cap / a.block);
-  unsigned char* ring = body + w * (DEPTH * F::SLOT) + lane * 16;
-
-  auto issue = [&](int chunk, int sub, int slot) {
-    unsigned char* dst = ring + slot * F::SLOT;
-    if (chunk < c1) {
-      if (sub < F::NK) {
+  const float *ks = a.ks + hd * a.blocks, *vs = a.vs + hd * a.blocks;
+  const int quad = w & 3, key_lane = quad * 32 + lane, st = tid - 64;  // tensor memory lane; thread of the softmax's 128
+  constexpr int RW = R / 4;  // query rows of a softmax warp: quad, quad + 4, ..; a lane holds dims 128 i + 4 lane .. + 3
+  uint2 q[RW][MT];
+  if (w >= 2) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = chunk * CHUNK + 16 * (g >> 1) + 2 * i + (g & 1);
-          if (D % 64 && sub == F::NK - 1)
-            cp_async8_zfill(dst + i * 512, kp + (key < top ? (size_t)key * D + sub * 64 + t * 8 : 0), key < top);
-          else
-            cp_async16_zfill(dst + i * 512, kp + (key < top ? (size_t)key * D + sub * 64 + t * 16 : 0), key < top);
-        }
-      } else {
-        const int key = chunk * CHUNK + 16 * t;
+    for (int j = 0; j < RW; ++j) {
+      const int row = row0 + quad + 4 * j;
+      const bool in = token_of(a, row) < a.mask.tokens;
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q) + row_at(a, b, h, row, a.qb, a.qt, a.qh) + lane * 4;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int d = (sub - F::NK) * 64 + i * 8 + g;
-          if (D % 64 == 0 || d < D)
-            cp_async16_zfill(dst + i * 512, vp + (key < top ? (size_t)d * a.cap + key : 0), key < top);
-        }
-      }
-    }
-    cp_async_commit();
-  };
-  // first pieces on their way before anything else is read
-#pragma unroll
-  for (int i = 0; i < DEPTH - 1; ++i) issue(c0 + w + (i / F::NSUB) * WARPS, i % F::NSUB, i);
-
-  // queries: limits, power-of-two row scales, f16 fragments
-  for (int r = w; r < ROWS; r += WARPS) {
-    const int row = row0 + r, tok = row / a.group;
-    const bool on = r < nrows;
-    const long long qo = b * a.qb + tok * a.qt + (h * a.group + row % a.group) * a.qh;
-    float x[D / 32], m = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      x[i] = on ? load16(a.q, qo + i * 32 + lane, a.half) : 0.f;
-      m = fmaxf(m, fabsf(x[i]));
-    }
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float p2 = row_pow2(m), inv = 1.0f / p2;
-    if (lane == 0) {
-      rowscale[r] = p2 * a.scale_log2;
-      rowlim[r] = on ? a.mask.limit(n, nq, pre, tok) : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      // element d = 64 c + 16 tq + 4 s + j (tail of 32 dims: 64 c + 8 tq + 4 s + j) of fragment step 4 c + s
-      const int d = i * 32 + lane, c = d / 64, r64 = d % 64;
-      const bool tail = D % 64 && c == F::NK - 1;
-      const int tq = tail ? r64 / 8 : r64 / 16, s = tail ? (r64 / 4) % 2 : (r64 / 4) % 4, j = d % 4;
-      // registers a0: row g, j 0..1; a1: row g + 8, j 0..1; a2: row g, j 2..3; a3: row g + 8, j 2..3
-      __half* f = reinterpret_cast<__half*>(qf + (c * 4 + s) * 32 + (r & 7) * 4 + tq);
-      f[((j >> 1) * 2 + (r >> 3)) * 2 + (j & 1)] = __float2half(x[i] * inv);
+      for (int i = 0; i < MT; ++i) q[j][i] = in && i * 128 + lane * 4 < a.dim ? ldg_row4(p + i * 128) : make_uint2(0, 0);
     }
   }
-  // largest V scale of the split: the probabilities carry vs / vref <= 1
-  float vref = 0.f;
-  for (int i = (c0 * CHUNK) / a.block + tid; i < a.cap / a.block && i * a.block < min(top, c1 * CHUNK); i += WARPS * 32)
-    vref = fmaxf(vref, vs[i]);
-  for (int o = 16; o > 0; o >>= 1) vref = fmaxf(vref, __shfl_xor_sync(0xffffffffu, vref, o));
-  if (lane == 0) red[w] = vref;
-  __syncthreads();
-  vref = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float vinv = vref > 0.f ? 1.0f / vref : 0.f;
-  const float rs0 = rowscale[g], rs1 = rowscale[g + 8];
-  const int lim0 = rowlim[g], lim1 = rowlim[g + 8];
-
-  float o[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-  int slot = 0;
-  // a lane's 16 keys lie in one block: one K and one V scale each chunk, fetched a chunk ahead
-  float kn = 0.f, vn = 0.f;
-  auto scales = [&](int chunk) {
-    const int key = chunk * CHUNK + 16 * t;
-    const bool live = chunk < c1 && key < top;  // whole 16-key pieces lie below the capacity
-    kn = live ? ks[key / a.block] : 0.f;
-    vn = live ? vs[key / a.block] : 0.f;
-  };
-  scales(c0 + w);
-  auto next = [&](int chunk, int sub) {  // piece `sub` of `chunk` has landed; fetch the one DEPTH - 1 ahead
-    cp_async_wait_group<DEPTH - 2>();
-    const int ahead = sub + DEPTH - 1;
-    issue(chunk + (ahead / F::NSUB) * WARPS, ahead % F::NSUB, slot == 0 ? DEPTH - 1 : slot - 1);
-    const unsigned char* src = ring + slot * F::SLOT;
-    slot = slot == DEPTH - 1 ? 0 : slot + 1;
-    return src;
-  };
-
-  for (int chunk = c0 + w; chunk < c1; chunk += WARPS) {
-    const int key0 = chunk * CHUNK + 16 * t;  // this lane's first key
-    const float kscale = kn, vfac = vn * vinv;
-    scales(chunk + WARPS);
-    float s[8][4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-#pragma unroll
-    for (int sub = 0; sub < F::NK; ++sub) {
-      const unsigned char* src = next(chunk, sub);
-      const bool tail = D % 64 && sub == F::NK - 1;
-      uint4 kr[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (tail) {
-          const uint2 x = *reinterpret_cast<const uint2*>(src + i * 512);
-          kr[i] = make_uint4(x.x, x.y, 0, 0);
-        } else {
-          kr[i] = *reinterpret_cast<const uint4*>(src + i * 512);
-        }
-      }
-#pragma unroll
-      for (int st = 0; st < (tail ? 2 : 4); ++st) {
-        const uint4 qa = qf[(sub * 4 + st) * 32 + lane];
-        const uint32_t qr[4] = {qa.x, qa.y, qa.z, qa.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t x = st == 0 ? kr[i].x : st == 1 ? kr[i].y : st == 2 ? kr[i].z : kr[i].w;
-          mma_f16(s[i], qr, e4m3x2_f16x2(x), e4m3x2_f16x2_hi(x));
-        }
-      }
-    }
-    // scores in log2 units, masked
-    const float f0 = rs0 * kscale, f1 = rs1 * kscale;
-    float mx0 = -INFINITY, mx1 = -INFINITY;
-    const bool whole = chunk * CHUNK + CHUNK <= low;  // seen by every row (rows behind the last are not stored)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int key = key0 + 2 * i + j;
-        s[i][j] = whole || key < lim0 ? s[i][j] * f0 : -INFINITY;
-        s[i][2 + j] = whole || key < lim1 ? s[i][2 + j] * f1 : -INFINITY;
-        mx0 = fmaxf(mx0, s[i][j]);
-        mx1 = fmaxf(mx1, s[i][2 + j]);
-      }
-    }
-#pragma unroll
-    for (int x = 1; x < 4; x <<= 1) {
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
-      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
-    }
-    const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
-    const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
-    if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
-      const float r0 = exp2_approx(m0 - b0), r1 = exp2_approx(m1 - b1);
-      l0 *= r0;
-      l1 *= r1;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        o[i][0] *= r0;
-        o[i][1] *= r0;
-        o[i][2] *= r1;
-        o[i][3] *= r1;
-      }
-      m0 = n0;
-      m1 = n1;
-    }
-    uint32_t p[4][4];
-    const float pf = vfac * 4096.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        s[i][j] = exp2_approx(s[i][j] - b0);
-        s[i][2 + j] = exp2_approx(s[i][2 + j] - b1);
-        l0 += s[i][j];
-        l1 += s[i][2 + j];
-      }
-      p[i >> 1][(i & 1) * 2] = pack_f16x2(s[i][0] * pf, s[i][1] * pf);
-      p[i >> 1][(i & 1) * 2 + 1] = pack_f16x2(s[i][2] * pf, s[i][3] * pf);
-    }
-    const int past = top - key0;  // V bytes from here on are behind every row's limit
-#pragma unroll
-    for (int sub = 0; sub < F::NV; ++sub) {
-      const unsigned char* src = next(chunk, F::NK + sub);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (sub * 64 + i * 8 >= D) break;
-        uint4 v = *reinterpret_cast<const uint4*>(src + i * 512);
-        if (past < 16) {
-          uint32_t* x = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int left = past - 4 * q;  // bytes of this word to keep
-            x[q] = left >= 4 ? x[q] : left <= 0 ? 0u : x[q] & ((1u << (8 * left)) - 1u);
-          }
-        }
-        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int st = 0; st < 4; ++st) mma_f16(o[sub * 8 + i], p[st], e4m3x2_f16x2(x[st]), e4m3x2_f16x2_hi(x[st]));
-      }
-    }
-  }
-  cp_async_wait_group<0>();
-#pragma unroll
-  for (int x = 1; x < 4; x <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, x);
-  }
-  if (t == 0) {
-    wml[w * ROWS + g] = make_float2(m0, l0);
-    wml[w * ROWS + g + 8] = make_float2(m1, l1);
-  }
-  __syncthreads();  // every warp is done with its ring
-  float* mo = reinterpret_cast<float*>(body) + w * ROWS * D;
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) {
-    *reinterpret_cast<float2*>(mo + g * D + i * 8 + 2 * t) = make_float2(o[i][0], o[i][1]);
-    *reinterpret_cast<float2*>(mo + (g + 8) * D + i * 8 + 2 * t) = make_float2(o[i][2], o[i][3]);
-  }
-  __syncthreads();
-  const size_t slot_id = (((size_t)b * a.heads + h) * a.tiles + tile) * a.nsplit + split;
-  const float unit = vref * (1.0f / 4096.0f);
-  for (int r = w; r < nrows; r += WARPS) {
-    float m = -INFINITY, l = 0.f, f[WARPS];
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) m = fmaxf(m, wml[i * ROWS + r].x);
-    const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) {
-      const float2 x = wml[i * ROWS + r];
-      f[i] = exp2_approx(x.x - base);
-      l += x.y * f[i];
-    }
-    const int row = row0 + r, lim = rowlim[r];
-    const long long oo = b * a.ob + (row / a.group) * a.ot + (h * a.group + row % a.group) * a.oh;
-    const float* src = reinterpret_cast<const float*>(body) + r * D;
-    const float norm = a.nsplit > 1 ? unit : lim > 0 ? unit / l : 0.f;
-    for (int d = lane * 2; d < D; d += 64) {
-      float x = 0.f, y = 0.f;
-#pragma unroll
-      for (int i = 0; i < WARPS; ++i) {
-        const float2 v = *reinterpret_cast<const float2*>(src + i * ROWS * D + d);
-        x += v.x * f[i];
-        y += v.y * f[i];
-      }
-      x *= norm;
-      y *= norm;
-      if (a.nsplit > 1) *reinterpret_cast<float2*>(a.part + (slot_id * ROWS + r) * D + d) = make_float2(x, y);
-      else if (lim > 0) store16x2(a.out, oo + d, x, y, a.half);
-      else store16x2(a.out, oo + d, 0.f, 0.f, a.half);
-    }
-    if (a.nsplit > 1 && lane == 0) a.ml[slot_id * ROWS + r] = make_float2(m, l);
-  }
-}
-
-// One warp per query row: o = sum_s 2^(m_s - m) part_s / sum_s 2^(m_s - m) l_s over the splits that the
-// row's tile has, in split order (the result does not depend on which split ended first).
-template <int D, int R>
-__global__ void merge_kernel(const AttnArgs a) {
-  const int lane = threadIdx.x & 31, h = blockIdx.y, b = blockIdx.z;
-  const int row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int n = a.mask.len(b), nq = a.mask.q_len(b), pre = a.mask.prefix ? a.mask.prefix[b] : 0;
-  if (row >= nq * a.group) return;
-  const int tile = row / R, r = row % R, last = min(tile * R + R, nq * a.group) - 1;
-  const int top = a.mask.limit(n, nq, pre, last / a.group), lim = a.mask.limit(n, nq, pre, row / a.group);
-  const int chunks = (top + CHUNK - 1) / CHUNK;
-  const int used = max(1, (chunks + a.split_chunks - 1) / a.split_chunks);
-  const size_t slot = (((size_t)b * a.heads + h) * a.tiles + tile) * a.nsplit;
-  float m = -INFINITY, l = 0.f;
-  for (int s = lane; s < used; s += 32) m = fmaxf(m, a.ml[(slot + s) * R + r].x);
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float base = m == -INFINITY ? 0.f : m;
-  float acc[D / 32] = {};
-  for (int s = 0; s < used; ++s) {
-    const float2 x = a.ml[(slot + s) * R + r];
-    const float f = exp2_approx(x.x - base);
-    l += x.y * f;
-    const float* p = a.part + ((slot + s) * R + r) * D + lane;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] += f * p[i * 32];
+  const int nrows = min(R, nq * a.group - row0);
+  if (nrows <= 0) return;  // of all CTAs of a cluster
+  // limits grow with the token: the tile's last row sees the most
+  const int top = a.mask.limit(n, nq, pre, token_of(a, row0 + nrows - 1));
+  const int low = a.mask.limit(n, nq, pre, token_of(a, row0));
+  const int all = (top + TILE - 1) / TILE, each = a.cluster ? (all + a.nsplit - 1) / a.nsplit : a.split_chunks;
+  const int t0 = split * each, nt = min(all, t0 + each) - t0;
+  launch_dependents();
+  const size_t slot_id = (((size_t)b * a.heads + h) * a.tiles + tile) * a.nsplit + split;
+  if (nt <= 0) {
+    if (a.cluster) {  // nothing left for this split
+      if (tid < R) mls[tid] = make_float2(-INFINITY, 0.f);
+      cluster_join<HALF, MT>(a, osum, PITCH, reinterpret_cast<const float*>(mls), 2, split, b, h, row0, nrows, n, nq, pre);
+    } else if (split == 0) {  // no key for any of these rows: split 0 says so
+      for (int i = tid; i < nrows * a.dim; i += THREADS) {
+        const int r = i / a.dim, d = i % a.dim;
+        if (a.nsplit > 1) a.part[(slot_id * R + r) * a.dim + d] = 0.f;
+        else store16(a.out, row_at(a, b, h, row0 + r, a.ob, a.ot, a.oh) + d, 0.f, HALF);
+      }
+      if (a.nsplit > 1 && tid < nrows) a.ml[slot_id * R + tid] = make_float2(-INFINITY, 0.f);
+    }
+    return;
   }
-  const float norm = 1.0f / l;
-  const long long oo = b * a.ob + (row / a.group) * a.ot + (h * a.group + row % a.group) * a.oh + lane;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    const float x = lim > 0 ? acc[i] * norm : 0.f;
-    if (a.half) reinterpret_cast<__half*>(a.out)[oo + i * 32] = __float2half(x);
-    else reinterpret_cast<bf16*>(a.out)[oo + i * 32] = __float2bfloat16(x);
+
+  if (tid == 0) {
+    for (int i = 0; i < C::SLOTS; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(sfull + i, 1);
+      mbar_init(sfree + i, 4);
+      mbar_init(pfull + i, 128);
+      mbar_init(pvdone + i, 1);
+      mbar_init(seen + i, 4);
+    }
+    mbar_init(maxes, 4);
+    *err = 0;
+    fence_mbar_init();
+    produce<1, C::SLOTS, MT>(ring, full, empty, &kmap, &vmap, t0, nt, (int)hd, err, 0, min(C::SLOTS, 2 * nt));
   }
+  if (w == 1) {
+    tmem_alloc(tmem_ptr, C::COLS);
+    tmem_relinquish();
+  }
+  // scales of this thread's key in the first tile, and the largest V scale of the split
+  float k_first = 0.f, v_first = 0.f, vref = 0.f;
+  if (w >= 2) {
+    const int key = t0 * TILE + key_lane;
+    if (key < top) {
+      k_first = ldg_now(ks + (key >> a.block_log2));
+      v_first = ldg_now(vs + (key >> a.block_log2));
+    }
+    const int kend = min(top, (t0 + nt) * TILE);
+    for (int i = ((t0 * TILE) >> a.block_log2) + st; (i << a.block_log2) < kend; i += 128) vref = fmaxf(vref, vs[i]);
+    // queries: limits, power-of-two row scales, E4M3 parts; rows behind the last are zero
+#pragma unroll
+    for (int j = 0; j < RW; ++j) {
+      const int r = quad + 4 * j;
+      const bool on = r < nrows;
+      float x[MT][4], m = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const float2 u = pair_f32<HALF>(q[j][i].x), v = pair_f32<HALF>(q[j][i].y);
+        x[i][0] = u.x, x[i][1] = u.y, x[i][2] = v.x, x[i][3] = v.y;
+        m = fmaxf(m, fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(v.x), fabsf(v.y))));
+      }
+      m = warp_max(m);
+      float back;
+      const float up = row_factor(m, back), mul = on ? up : 0.f;
+      if (lane == 0) {
+        rowscale[r] = back * a.scale_log2;
+        rowlim[r] = on ? a.mask.limit(n, nq, pre, token_of(a, row0 + r)) : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        float y[4] = {x[i][0] * mul, x[i][1] * mul, x[i][2] * mul, x[i][3] * mul};
+        split_query<C::QP>(y, 16.f, [&](int p, uint32_t e) {
+          *reinterpret_cast<uint32_t*>(qs + i * C::NS * 128 + swz(p * R + r, lane * 4)) = e;
+        });
+      }
+    }
+    // columns that pad the products to 16: never read, but kept finite
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      for (int j = st; j < (C::NS - C::QP * R) * 8; j += 128)
+        *reinterpret_cast<uint4*>(qs + i * C::NS * 128 + C::QP * R * 128 + j * 16) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      for (int j = st; j < (C::NP - C::PP * R) * 8; j += 128)
+        *reinterpret_cast<uint4*>(ps + i * C::PBYTES + C::PP * R * 128 + j * 16) = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_shared();
+    vref = warp_max(vref);
+    if (lane == 0) red[quad] = vref;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_ptr;
+  const uint32_t tmem_o = tmem + 2 * C::NS;
+
+  if (w == 0) {
+    if (lane == 0) produce<1, C::SLOTS, MT>(ring, full, empty, &kmap, &vmap, t0, nt, (int)hd, err, min(C::SLOTS, 2 * nt), 2 * nt);
+    __syncwarp();
+  } else if (w == 1) {
+    const int steps = a.dim / 32;
+    constexpr uint32_t ids = idesc_f8(C::NS, false, false), idp = idesc_f8(C::NP, false, true);
+    const uint32_t qb = desc_lo(qs), pb = desc_lo(ps);
+    bool ok = true;
+    auto scores = [&](int i) {
+      const int pos = pos_k<1>(i), slot = pos % C::SLOTS;
+      ok = ok && mbar_wait(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
+      ok = ok && (i < 2 || mbar_wait(sfree + (i & 1), ((i >> 1) - 1) & 1, err, ERR_SFREE));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      tc_fence_after();
+      const uint32_t ka = desc_lo(ring + slot * C::SLOT), d = tmem + (i & 1) * C::NS;
+#pragma unroll
+      for (int k = 0; k < MT * 4; ++k)
+        if (k < steps) mma_f8(d, ka + (k >> 2) * 1024 + (k & 3) * 2, qb + (k >> 2) * C::NS * 8 + (k & 3) * 2, ids, k > 0);
+      tc_commit_elect(sfull + (i & 1));
+      tc_commit_elect(empty + slot);
+    };
+    scores(0);
+    for (int i = 0; i < nt && ok; ++i) {
+      if (i + 1 < nt) scores(i + 1);
+      const int pos = pos_v<1>(i, nt), slot = pos % C::SLOTS;
+      ok = ok && mbar_wait(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
+      ok = ok && mbar_wait(pfull + (i & 1), (i >> 1) & 1, err, ERR_P);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t va = desc_lo(ring + slot * C::SLOT), pi = pb + (i & 1) * (C::PBYTES / 16);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_f8(tmem_o + m * C::NP, va + m * 1024 + k * 2, pi + k * 2, idp, i > 0 || k > 0);
+      tc_commit_elect(pvdone + (i & 1));
+      tc_commit_elect(empty + slot);
+    }
+  } else {
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    vref = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float vinv = vref > 0.f ? kPTop / vref : 0.f;
+
+    float m[R], l[R], rs[R];  // the subtracted maximum (the same in all threads), this key lane's sum, the rows' scales
+#pragma unroll
+    for (int r = 0; r < R; ++r) m[r] = -INFINITY, l[r] = 0.f, rs[r] = rowscale[r];
+    float kn = k_first, vn = v_first;
+    int grown = 0;  // times that the maximum moved
+    auto scales = [&](int i) {
+      const int key = (t0 + i) * TILE + key_lane;
+      const bool live = i < nt && key < top;
+      kn = live ? ks[key >> a.block_log2] : 0.f;
+      vn = live ? vs[key >> a.block_log2] : 0.f;
+    };
+    bool ok = true;
+    for (int i = 0; i < nt; ++i) {
+      const int key = (t0 + i) * TILE + key_lane;
+      const float kscale = kn, vfac = vn * vinv;
+      scales(i + 1);
+      ok = mbar_wait(sfull + (i & 1), (i >> 1) & 1, err, ERR_S);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      float s[R];
+      {
+        const uint32_t ts = tmem + lanes + (i & 1) * C::NS;
+        float v[C::NS];
+#pragma unroll
+        for (int c = 0; c < C::NS; c += 16) tmem_ld16(ts + c, v + c);
+        tc_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sfree + (i & 1));
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          s[r] = v[r] + v[R + r] * 0.0625f;
+          if (HALF) s[r] += v[(C::QP - 1) * R + r] * (1.0f / 256.0f);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[r] *= rs[r] * kscale;
+      if ((t0 + i) * TILE + TILE > low) {  // not seen by every row
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r] = key < rowlim[r] ? s[r] : -INFINITY;
+      }
+      bool grew = false;
+#pragma unroll
+      for (int r = 0; r < R; ++r) grew |= s[r] > m[r] + kLag;
+      grew = __any_sync(0xffffffffu, grew);
+      if (lane == 0) {
+        flags[(i & 1) * 4 + quad] = grew;
+        mbar_arrive(seen + (i & 1));
+      }
+      ok = mbar_wait(seen + (i & 1), (i >> 1) & 1, err, ERR_SEEN);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const int4 fl = *reinterpret_cast<const int4*>(flags + (i & 1) * 4);
+      if (fl.x | fl.y | fl.z | fl.w) {  // the same in all 128 threads
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float x = warp_max(s[r]);
+          if (lane == 0) wmax[quad * R + r] = x;
+        }
+        if (lane == 0) mbar_arrive(maxes);
+        ok = mbar_wait(maxes, grown & 1, err, ERR_SEEN);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++grown;
+        float f[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float x = fmaxf(m[r], fmaxf(fmaxf(wmax[r], wmax[R + r]), fmaxf(wmax[2 * R + r], wmax[3 * R + r])));
+          f[r] = x == -INFINITY ? 1.f : exp2_approx(m[r] - x);
+          m[r] = x;
+          l[r] *= f[r];
+        }
+        if (i > 0) {
+          ok = mbar_wait(pvdone + ((i - 1) & 1), ((i - 1) >> 1) & 1, err, ERR_PV);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int c = 0; c < C::NP; c += 16) {
+              float v[16];
+              uint32_t u[16];
+              tmem_ld16(tmem_o + lanes + mt * C::NP + c, v);
+              tc_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(c + j < C::PP * R ? v[j] * f[(c + j) % R] : v[j]);
+              tmem_st16(tmem_o + lanes + mt * C::NP + c, u);
+            }
+          tc_wait_st();
+          tc_fence_before();
+        }
+      }
+      if (i >= 2) {
+        ok = mbar_wait(pvdone + (i & 1), ((i >> 1) - 1) & 1, err, ERR_PV);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
+      unsigned char* pb = ps + (i & 1) * C::PBYTES;
+#pragma unroll
+      for (int r = 0; r < R; r += 2) {
+        const float x = exp2_approx(s[r] - (m[r] == -INFINITY ? 0.f : m[r]));
+        const float y = exp2_approx(s[r + 1] - (m[r + 1] == -INFINITY ? 0.f : m[r + 1]));
+        l[r] += x;
+        l[r + 1] += y;
+        uint32_t p = pack_f16x2(x * vfac, y * vfac);
+        if (!HALF) p = round9(p);
+#pragma unroll
+        for (int k = 0; k < C::PP; ++k) {
+          pb[swz(k * R + r, key_lane)] = (unsigned char)(p >> 8);
+          pb[swz(k * R + r + 1, key_lane)] = (unsigned char)(p >> 24);
+          if (k + 1 < C::PP) p = rest8(p);
+        }
+      }
+      const int left = top - (t0 + i) * TILE;
+      if (left < TILE) {
+        // keys behind the last limit have P = 0, but their V codes may be NaN: clear them in the tile
+        const int pos = pos_v<1>(i, nt), slot = pos % C::SLOTS;
+        ok = mbar_wait(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        clear_behind(ring + slot * C::SLOT, MT * 128, left, st, 128);
+      }
+      fence_proxy_async_shared();
+      mbar_arrive(pfull + (i & 1));
+    }
+    if (ok) ok = mbar_wait(pvdone + ((nt - 1) & 1), ((nt - 1) >> 1) & 1, err, ERR_PV);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    // sums of the rows over the 128 key lanes: through the free P buffers, a warp adds up each fourth row
+    float* ls = reinterpret_cast<float*>(ps);
+#pragma unroll
+    for (int r = 0; r < R; ++r) ls[r * 128 + st] = l[r];
+    bar_softmax();
+#pragma unroll
+    for (int j = 0; j < RW; ++j) {
+      const int r = quad + 4 * j;
+      float x = (ls[r * 128 + lane] + ls[r * 128 + 32 + lane]) + (ls[r * 128 + 64 + lane] + ls[r * 128 + 96 + lane]);
+      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      float top_m = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < R; ++k) top_m = k == r ? m[k] : top_m;
+      if (lane == 0) {
+        mls[r] = make_float2(top_m, x);
+        if (a.nsplit > 1 && !a.cluster && r < nrows) a.ml[slot_id * R + r] = make_float2(top_m, x);
+      }
+    }
+    bar_softmax();
+    const float unit = vref * (1.0f / kPTop);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float v[C::NP];
+#pragma unroll
+      for (int c = 0; c < C::NP; c += 16) tmem_ld16(tmem_o + lanes + mt * C::NP + c, v + c);
+      tc_wait_ld();
+      const int d = mt * 128 + key_lane;
+      if (d < a.dim) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          if (r >= nrows) break;
+          float x = v[r] + v[R + r] * 0.125f + v[2 * R + r] * (1.0f / 64.0f);
+          if (HALF) x += v[(C::PP - 1) * R + r] * (1.0f / 512.0f);
+          x = ok ? x * unit : __int_as_float(0x7fffffff);  // a wait that ran out is seen in the result
+          if (a.cluster) osum[r * PITCH + d] = x;
+          else if (a.nsplit > 1) a.part[(slot_id * R + r) * a.dim + d] = x;
+          else store16(a.out, row_at(a, b, h, row0 + r, a.ob, a.ot, a.oh) + d, rowlim[r] > 0 ? x / mls[r].y : 0.f, HALF);
+        }
+      }
+      __syncwarp();
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (w == 1) tmem_dealloc(tmem, C::COLS);
+  if (a.cluster) cluster_join<HALF, MT>(a, osum, PITCH, reinterpret_cast<const float*>(mls), 2, split, b, h, row0, nrows, n, nq, pre);
 }
 
-template <int D>
-fa_status launch(const AttnArgs& a, int batch, cudaStream_t s) {
-  FA_CUDA(nullptr, cudaFuncSetAttribute(few_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<D>::SMEM));
-  few_kernel<D><<<dim3(a.nsplit * a.tiles, a.heads, batch), WARPS * 32, Few<D>::SMEM, s>>>(a);
-  FA_CUDA(nullptr, cudaGetLastError());
-  if (a.nsplit > 1) {
-    merge_kernel<D, ROWS><<<dim3((a.mask.tokens * a.group + 3) / 4, a.heads, batch), 128, 0, s>>>(a);
-    FA_CUDA(nullptr, cudaGetLastError());
-  }
-  return FA_OK;
+template <int R, bool HALF, int MT>
+fa_status launch(const AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
+  constexpr int SMEM = Cfg<R, HALF, MT>::SMEM;
+  FA_CUDA(nullptr, cudaFuncSetAttribute(few_kernel<R, HALF, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+  return kv8_launch(few_kernel<R, HALF, MT>, a, batch, THREADS, SMEM, km, vm, s);
+}
+template <int R>
+fa_status launch_rows(const AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
+  if (a.dim <= 128) return a.half ? launch<R, true, 1>(a, batch, km, vm, s) : launch<R, false, 1>(a, batch, km, vm, s);
+  return a.half ? launch<R, true, 2>(a, batch, km, vm, s) : launch<R, false, 2>(a, batch, km, vm, s);
 }
 
 }  // namespace
 
-fa_status kv8_launch_few(const AttnArgs& a, int dim, int batch, cudaStream_t s) {
-  switch (dim) {
-    case 64: return launch<64>(a, batch, s);
-    case 96: return launch<96>(a, batch, s);
-    case 128: return launch<128>(a, batch, s);
-    default: return launch<256>(a, batch, s);
-  }
+fa_status kv8_launch_few(const AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
+  return a.rows == 8 ? launch_rows<8>(a, batch, km, vm, s) : launch_rows<16>(a, batch, km, vm, s);
 }

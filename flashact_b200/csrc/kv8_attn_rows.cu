@@ -1,0 +1,416 @@
+// Attention over the 8-bit cache for many query rows of a key head, 128 at a time, on the tensor cores' 8-bit kind; bound
+// by their rate.
+//
+// o = sum_j p_j vs_j V_j / sum_j p_j with p_j = 2^(s_j - max s), s_j = log2(e) scale ks_j (q . K_j). The cache's codes go into both
+// products as TMA brings them, S = Q K^T and O = P V; queries and probabilities, which have more than eight bits, are
+// sums of 8-bit parts, each the rounding of what the parts before it left over, and every part is one more product into the same sums:
+//   queries  two E4M3 parts (three for fp16) of a row scaled by a power of two to [128, 256): off by at most 2^-10, that is 2^-17 of
+//            the row's largest element, where E4M3's smallest steps end it;
+//   P        three E5M2 parts (four for fp16) of p * 2^14 * vs / (the split's largest vs) rounded to f16: 2^-10 of each p
+//            (fp16: 2^-11) and no less than 2^-31 of the largest.
+// That is 2 + 3 products at the 8-bit rate against the 2 + 2 that one bf16 product each would cost at half that rate,
+// without converting the cache or holding it in 16 bits in shared memory, whose bandwidth would bound it.
+//
+// P goes to tensor memory, whence the second product reads it as its first operand: shared memory then holds the queries' parts and
+// five slots of K and V tiles at head_dim 256 (with P in shared memory three, and the products waited for tiles).
+//
+// Warp 0 keeps a ring of K and V tiles (128 keys) full, warp 1 issues the products (scores of tile i + 2 before P V
+// of tile i), warps 2..9 turn scores into probabilities: a thread has one query row and half of the tile's keys, and the two
+// threads of a row exchange their maxima, those of tile i + 1 while they write P of tile i. The running maximum moves only where it grew by more than 2^1, the only
+// case that touches O.
+#include "kv8_tc.cuh"
+
+namespace {
+
+using namespace fa;
+using namespace fa::kv8;
+
+constexpr int THREADS = 320, ROWS = 128;
+constexpr float kPTop = 16384.0f;  // p = 1; with a maximum that lags by up to kLag, 2^15 (E5M2 ends at 57344)
+constexpr float kLag = 1.0f;
+
+template <bool HALF, int MT_>
+struct Cfg {
+  static constexpr int MT = MT_;
+  static constexpr int QP = HALF ? 3 : 2, PP = HALF ? 4 : 3;
+  static constexpr int SLOT = MT * 16384, QBYTES = QP * MT * 16384;
+  static constexpr int STATE = 3072, REST = QBYTES + STATE;
+  static constexpr int SLOTS_ = (227 * 1024 - REST) / SLOT, SLOTS = SLOTS_ > 8 ? 8 : SLOTS_;
+  static constexpr int SMEM = REST + SLOTS * SLOT;
+  static_assert(ROWS * (MT * 128 + 4) * 4 <= SLOTS * SLOT + QBYTES, "sums of a split");
+  static_assert(SLOTS >= 2, "shared memory");  // K and V of a tile; scores of the next need K's slot only
+};
+
+__device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+template <bool HALF, int MT>
+__global__ void __launch_bounds__(THREADS, 1)
+    rows_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using C = Cfg<HALF, MT>;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  unsigned char* ring = smem;
+  unsigned char* qs = smem + C::SLOTS * C::SLOT;  // [part][MT][128][128]
+  unsigned char* state = qs + C::QBYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(state);  // [SLOTS] tile has landed
+  uint64_t* empty = full + C::SLOTS;                    // [SLOTS] its products are done
+  uint64_t* sfull = empty + C::SLOTS;                   // scores are in tensor memory
+  uint64_t* sfree = sfull + 1;                          // and have been read
+  uint64_t* pfull = sfree + 1;                          // probabilities are in tensor memory
+  uint64_t* pvdone = pfull + 1;                         // and their product is done
+  uint64_t* seen = pvdone + 1;                          // the eight warps' maxima are in half_max
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(seen + 1);
+  volatile int* err = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  float* red = reinterpret_cast<float*>(state + 256);       // [8]
+  float* half_max = reinterpret_cast<float*>(state + 512);  // [2][2][128], a tile's maxima in the one of its parity
+  float* rowscale = half_max + 2 * ROWS;                    // [128], read before the second tile's maxima
+  float* osum = reinterpret_cast<float*>(smem);             // [128][PITCH] sums of the split and, behind a row, its maximum and sum
+  constexpr int PITCH = MT * 128 + 4;
+
+  const int tid = threadIdx.x, w = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int split = blockIdx.x % a.nsplit, tile = blockIdx.x / a.nsplit, h = blockIdx.y, b = blockIdx.z;
+  const int row0 = tile * ROWS;
+  const size_t hd = ((size_t)b * a.layers + a.layer) * a.heads + h;
+  const float *ks = a.ks + hd * a.blocks, *vs = a.vs + hd * a.blocks;
+  const int n = a.mask.len(b), nq = a.mask.q_len(b), pre = a.mask.prefix ? a.mask.prefix[b] : 0;
+  const int nrows = min(ROWS, nq * a.group - row0);
+  if (nrows <= 0) return;  // of all CTAs of a cluster
+  // limits grow with the token: the tile's last row sees the most
+  const int top = a.mask.limit(n, nq, pre, token_of(a, row0 + nrows - 1));
+  const int low = a.mask.limit(n, nq, pre, token_of(a, row0));
+  const int all = (top + TILE - 1) / TILE, each = a.cluster ? (all + a.nsplit - 1) / a.nsplit : a.split_chunks;
+  const int t0 = split * each, nt = min(all, t0 + each) - t0;
+  launch_dependents();
+  const size_t slot_id = (((size_t)b * a.heads + h) * a.tiles + tile) * a.nsplit + split;
+  if (nt <= 0) {
+    if (a.cluster) {  // nothing left for this split
+      if (tid < ROWS) *reinterpret_cast<float2*>(osum + tid * PITCH + MT * 128) = make_float2(-INFINITY, 0.f);
+      cluster_join<HALF, MT>(a, osum, PITCH, osum + MT * 128, PITCH, split, b, h, row0, nrows, n, nq, pre);
+    } else if (split == 0) {  // no key for any of these rows: split 0 says so
+      for (int i = tid; i < nrows * a.dim; i += THREADS) {
+        const int r = i / a.dim, d = i % a.dim;
+        if (a.nsplit > 1) a.part[(slot_id * ROWS + r) * a.dim + d] = 0.f;
+        else store16(a.out, row_at(a, b, h, row0 + r, a.ob, a.ot, a.oh) + d, 0.f, HALF);
+      }
+      if (a.nsplit > 1 && tid < nrows) a.ml[slot_id * ROWS + tid] = make_float2(-INFINITY, 0.f);
+    }
+    return;
+  }
+
+  if (tid == 0) {
+    for (int i = 0; i < C::SLOTS; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    mbar_init(sfull, 1);
+    mbar_init(sfree, 8);
+    mbar_init(pfull, 256);
+    mbar_init(pvdone, 1);
+    mbar_init(seen, 8);
+    *err = 0;
+    fence_mbar_init();
+    produce<2, C::SLOTS, MT>(ring, full, empty, &kmap, &vmap, t0, nt, (int)hd, err, 0, min(C::SLOTS, 2 * nt));
+  }
+  if (w == 1) {
+    tmem_alloc(tmem_ptr, 512);
+    tmem_relinquish();
+  }
+  float vref = 0.f;  // largest V scale of the split
+  if (w >= 2) {
+    const int kend = min(top, (t0 + nt) * TILE);
+    for (int i = ((t0 * TILE) >> a.block_log2) + tid - 64; (i << a.block_log2) < kend; i += 256) vref = fmaxf(vref, vs[i]);
+    // queries: power-of-two row scales and E4M3 parts; rows behind the last are zero
+    constexpr int LANES = MT * 16, PER = 32 / LANES, N = 16 / PER;  // lanes of a row, rows at a time, such groups of the warp's 16 rows
+    const int l8 = (lane % LANES) * 8;                              // this lane's dims, l8 .. + 7
+    auto source = [&](int j) {
+      const int r = row0 + (w - 2) * 16 + j * PER + lane / LANES;
+      return token_of(a, r) < a.mask.tokens && l8 < a.dim
+                 ? reinterpret_cast<const uint16_t*>(a.q) + row_at(a, b, h, r, a.qb, a.qt, a.qh) + l8 : nullptr;
+    };
+    auto split = [&](int j, uint4 q) {
+      const int r = (w - 2) * 16 + j * PER + lane / LANES;
+      const float2 x0 = pair_f32<HALF>(q.x), x1 = pair_f32<HALF>(q.y), x2 = pair_f32<HALF>(q.z), x3 = pair_f32<HALF>(q.w);
+      float m = fmaxf(fmaxf(fmaxf(fabsf(x0.x), fabsf(x0.y)), fmaxf(fabsf(x1.x), fabsf(x1.y))),
+                      fmaxf(fmaxf(fabsf(x2.x), fabsf(x2.y)), fmaxf(fabsf(x3.x), fabsf(x3.y))));
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      float back;
+      const float up = row_factor(m, back), mul = r < nrows ? copysignf(up, a.scale_log2) : 0.f;
+      if (l8 == 0) rowscale[r] = back * fabsf(a.scale_log2);
+      float y[4] = {x0.x * mul, x0.y * mul, x1.x * mul, x1.y * mul}, z[4] = {x2.x * mul, x2.y * mul, x3.x * mul, x3.y * mul};
+      uint32_t e[C::QP];
+      split_query<C::QP>(y, 1.f, [&](int p, uint32_t v) { e[p] = v; });
+      split_query<C::QP>(z, 1.f, [&](int p, uint32_t v) {
+        *reinterpret_cast<uint2*>(qs + (p * MT + (l8 >> 7)) * 16384 + swz(r, l8 & 127)) = make_uint2(e[p], v);
+      });
+    };
+    if (a.q_wide) {  // all loads on their way first
+      uint4 q[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const uint16_t* p = source(j);
+        q[j] = p ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) split(j, q[j]);
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < N; ++j) {
+        const uint16_t* p = source(j);
+        uint32_t u[4] = {0, 0, 0, 0};
+        if (p) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) u[k] = (uint32_t)__ldg(p + 2 * k) | ((uint32_t)__ldg(p + 2 * k + 1) << 16);
+        }
+        __syncwarp();
+        split(j, make_uint4(u[0], u[1], u[2], u[3]));
+      }
+    }
+    fence_proxy_async_shared();
+    vref = warp_max(vref);
+    if (lane == 0) red[w - 2] = vref;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_o = *tmem_ptr, tmem_s = tmem_o + 256, tmem_p = tmem_o + 384;  // O, scores, parts of P (32 columns each)
+
+  if (w == 0) {
+    if (lane == 0) produce<2, C::SLOTS, MT>(ring, full, empty, &kmap, &vmap, t0, nt, (int)hd, err, min(C::SLOTS, 2 * nt), 2 * nt);
+    __syncwarp();
+  } else if (w == 1) {
+    const int steps = a.dim / 32;
+    const uint32_t ids = idesc_f8(TILE, false, false), idp = idesc_f8(a.dim, true, false);
+    const uint32_t qa = desc_lo(qs);
+    bool ok = true;
+    auto scores = [&](int i) {
+      const int pos = pos_k<2>(i), slot = pos % C::SLOTS;
+      ok = ok && mbar_wait(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
+      ok = ok && (i < 1 || mbar_wait(sfree, (i - 1) & 1, err, ERR_SFREE));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      tc_fence_after();
+      const uint32_t kb = desc_lo(ring + slot * C::SLOT);
+#pragma unroll
+      for (int p = 0; p < C::QP; ++p)
+#pragma unroll
+        for (int k = 0; k < MT * 4; ++k)
+          if (k < steps) mma_f8(tmem_s, qa + (p * MT + (k >> 2)) * 1024 + (k & 3) * 2, kb + (k >> 2) * 1024 + (k & 3) * 2, ids, p > 0 || k > 0);
+      tc_commit_elect(sfull);
+      tc_commit_elect(empty + slot);
+    };
+    scores(0);
+    if (nt > 1 && ok) scores(1);
+    for (int i = 0; i < nt && ok; ++i) {
+      if (i + 2 < nt) scores(i + 2);  // scores i + 1 have been read by then, before P of tile i is there
+      ok = ok && mbar_wait(pfull, i & 1, err, ERR_P);
+      const int pos = pos_v<2>(i, nt), slot = pos % C::SLOTS;
+      ok = ok && mbar_wait(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t vb = desc_lo(ring + slot * C::SLOT);
+#pragma unroll
+      for (int p = 0; p < C::PP; ++p)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_f8_ts(tmem_o, tmem_p + p * 32 + k * 8, vb + k * 2, idp, i > 0 || p > 0 || k > 0);
+      tc_commit_elect(pvdone);
+      tc_commit_elect(empty + slot);
+    }
+  } else {
+    const int sw = w - 2, half = sw >> 2, quad = w & 3, row = quad * 32 + lane, st = tid - 64;
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vref = fmaxf(vref, red[i]);
+    const float vinv = vref > 0.f ? kPTop / vref : 0.f;
+    const float rs = rowscale[row];
+    const int lim = row < nrows ? a.mask.limit(n, nq, pre, token_of(a, row0 + row)) : 0;
+
+    float kn[4], vn[4];  // scales of the four 16-key groups of this half, a tile ahead
+    auto scales = [&](int i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = (t0 + i) * TILE + half * 64 + 16 * j;
+        const bool live = i < nt && key < top;
+        kn[j] = live ? __ldg(ks + (key >> a.block_log2)) : 0.f;
+        vn[j] = live ? __ldg(vs + (key >> a.block_log2)) : 0.f;
+      }
+    };
+    scales(0);
+    float m = -INFINITY, l = 0.f;  // the subtracted maximum (the same in a row's two threads), this half's sum
+    bool ok = true;
+    // Raw scores s of a tile, factors f per 16-key group (the scale's sign went into the queries, so f >= 0 and a group's maximum
+    // is f times that of its scores), and this half's maximum on its way to the row's other thread. Masked scores are -inf.
+    float s[64], f[4], vf[4], mx;
+    auto fetch = [&](int i) {
+      ok = mbar_wait(sfull, i & 1, err, ERR_S);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 64; c += 16) tmem_ld16(tmem_s + lanes + half * 64 + c, s + c);
+      tc_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sfree);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[j] = rs * kn[j];
+        vf[j] = vn[j] * vinv;
+      }
+      if ((t0 + i) * TILE + TILE > low) {  // not seen by every row
+        const int left = lim - (t0 + i) * TILE - half * 64;
+#pragma unroll
+        for (int c = 0; c < 64; ++c) s[c] = c < left ? s[c] : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = f[j] == 0.f ? 1e-30f : f[j];  // -inf stays -inf
+      }
+      scales(i + 1);
+      mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float g = fmaxf(s[16 * j], s[16 * j + 1]);
+#pragma unroll
+        for (int c = 2; c < 16; c += 2) g = fmaxf(fmaxf(g, s[16 * j + c]), s[16 * j + c + 1]);
+        mx = fmaxf(mx, g * f[j]);
+      }
+      half_max[(i & 1) * 2 * ROWS + half * ROWS + row] = mx;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(seen);
+    };
+    fetch(0);
+    for (int i = 0; i < nt && ok; ++i) {
+      ok = mbar_wait(seen, i & 1, err, ERR_SEEN);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      mx = fmaxf(mx, half_max[(i & 1) * 2 * ROWS + (half ^ 1) * ROWS + row]);
+      const bool grew = mx > m + kLag || (m == -INFINITY && mx > m);
+      if (__any_sync(0xffffffffu, grew)) {  // the same in the row's other thread's warp
+        const float x = fmaxf(m, mx), down = x == -INFINITY ? 1.f : exp2_approx(m - x);
+        m = x;
+        l *= down;
+        if (i > 0) {  // O is at rest once the tile before is done
+          ok = mbar_wait(pvdone, (i - 1) & 1, err, ERR_PV);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          for (int c = half * 16; c < a.dim; c += 32) {
+            float v[16];
+            uint32_t u[16];
+            tmem_ld16(tmem_o + lanes + c, v);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(v[j] * down);
+            tmem_st16(tmem_o + lanes + c, u);
+          }
+          tc_wait_st();
+          tc_fence_before();
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      uint32_t e[C::PP][16];  // all of P before the wait for its place, which the product of the tile before still reads
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float* x = s + 16 * j + 4 * c;
+          const float x0 = exp2_approx(fmaf(x[0], f[j], -base)), x1 = exp2_approx(fmaf(x[1], f[j], -base));
+          const float x2 = exp2_approx(fmaf(x[2], f[j], -base)), x3 = exp2_approx(fmaf(x[3], f[j], -base));
+          l += (x0 + x1) + (x2 + x3);
+          uint32_t p = pack_f16x2(x0 * vf[j], x1 * vf[j]), q = pack_f16x2(x2 * vf[j], x3 * vf[j]);
+          if (!HALF) p = round9(p), q = round9(q);
+#pragma unroll
+          for (int k = 0; k < C::PP; ++k) {
+            e[k][4 * j + c] = __byte_perm(p, q, 0x7531);  // the upper bytes
+            if (k + 1 < C::PP) p = rest1(p), q = rest1(q);
+          }
+        }
+      if (i + 1 < nt) fetch(i + 1);
+      if (!ok) break;
+      if (i > 0) {
+        ok = mbar_wait(pvdone, (i - 1) & 1, err, ERR_PV);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
+      tc_fence_after();
+#pragma unroll
+      for (int k = 0; k < C::PP; ++k) tmem_st16(tmem_p + lanes + k * 32 + half * 16, e[k]);
+      const int left = top - (t0 + i) * TILE;
+      if (left < TILE) {
+        const int pos = pos_v<2>(i, nt), slot = pos % C::SLOTS;
+        ok = mbar_wait(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        clear_behind(ring + slot * C::SLOT, MT * 128, left, st, 256);
+        fence_proxy_async_shared();
+      }
+      tc_wait_st();
+      tc_fence_before();
+      mbar_arrive(pfull);
+    }
+    if (ok) ok = mbar_wait(pvdone, (nt - 1) & 1, err, ERR_PV);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    float* sums = half_max + (nt & 1) * 2 * ROWS;  // the maxima's buffer that the last tile did not use
+    sums[half * ROWS + row] = l;
+    bar_softmax();
+    l = sums[row] + sums[ROWS + row];
+    if (half == 0) {
+      if (a.cluster) *reinterpret_cast<float2*>(osum + row * PITCH + MT * 128) = make_float2(m, l);
+      else if (a.nsplit > 1 && row < nrows) a.ml[slot_id * ROWS + row] = make_float2(m, l);
+    }
+    const float unit = vref * (1.0f / kPTop);
+    const float norm = !ok ? __int_as_float(0x7fffffff)  // a wait that ran out is seen in the result
+                           : a.nsplit > 1 ? unit : lim > 0 ? unit / l : 0.f;
+    uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + row_at(a, b, h, row0 + row, a.ob, a.ot, a.oh);
+#pragma unroll 2
+    for (int c = half * 16; c < a.dim; c += 32) {
+      float v[16];
+      tmem_ld16(tmem_o + lanes + c, v);
+      tc_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = ok && lim <= 0 ? 0.f : v[j] * norm;
+      if (row >= nrows) {
+        // not a row of the call
+      } else if (a.nsplit > 1) {
+        float4* p = reinterpret_cast<float4*>(a.cluster ? osum + row * PITCH + c : a.part + (slot_id * ROWS + row) * a.dim + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      } else {
+        uint32_t u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const __nv_bfloat162 bv = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+          u[j] = HALF ? pack_f16x2(v[2 * j], v[2 * j + 1]) : *reinterpret_cast<const uint32_t*>(&bv);
+        }
+        if ((reinterpret_cast<uintptr_t>(out + c) & 15) == 0) {
+          reinterpret_cast<uint4*>(out + c)[0] = make_uint4(u[0], u[1], u[2], u[3]);
+          reinterpret_cast<uint4*>(out + c)[1] = make_uint4(u[4], u[5], u[6], u[7]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            out[c + 2 * j] = (uint16_t)u[j];
+            out[c + 2 * j + 1] = (uint16_t)(u[j] >> 16);
+          }
+        }
+      }
+      __syncwarp();
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (w == 1) tmem_dealloc(tmem_o, 512);
+  if (a.cluster) cluster_join<HALF, MT>(a, osum, PITCH, osum + MT * 128, PITCH, split, b, h, row0, nrows, n, nq, pre);
+}
+
+template <bool HALF, int MT>
+fa_status launch(const AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
+  constexpr int SMEM = Cfg<HALF, MT>::SMEM;
+  return kv8_launch(rows_kernel<HALF, MT>, a, batch, THREADS, SMEM, km, vm, s);
+}
+
+}  // namespace
+
+fa_status kv8_launch_rows(const AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
+  if (a.dim <= 128) return a.half ? launch<true, 1>(a, batch, km, vm, s) : launch<false, 1>(a, batch, km, vm, s);
+  return a.half ? launch<true, 2>(a, batch, km, vm, s) : launch<false, 2>(a, batch, km, vm, s);
+}

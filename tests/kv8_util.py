@@ -79,12 +79,22 @@ def attend(ref, layer, q, lens, *, causal=True, prefix=None, q_lens=None, scale=
     The tolerance counts roundings. Output: half a step of q's type, u |o|. Probabilities: rounded to eight bits
     (bf16 queries) or eleven (fp16) before the product, so each p_j is off by at most w p_j, and the output by
     w sum p |v| / sum p. Scores: fp32 sums of D products are off by at most (D + 8) 2^-23 of scale * sum |q k|
-    (the matrix unit truncates), 2^x by 2^-21 of its result: p_j is off by that share, in numerator and sum."""
+    (the matrix unit truncates), 2^x by 2^-21 of its result: p_j is off by that share, in numerator and sum.
+    Smallest probabilities: up to 16 rows of a key head (few), P is held as p_j 2^12 vs_j / max vs in f16 (steps of 2^-24 at
+    the small end, half of one is 2^-25) and from there in E5M2 parts, the third in units of 1/64 (steps of 2^-16, half of one
+    is 2^-17 / 64 = 2^-23): together each is off by at most 2^-22 whatever its size, which is 2^-34 of the largest. More rows: p_j 2^14
+    and parts in the same units: 2^-17 + 2^-25 < 2^-16, which is 2^-30 of the largest. The output is off by that times
+    sum max vs |code_j| / sum 2^(s_j - max s), the sum being relative to a maximum no larger than the true one.
+    Smallest query elements: parts of a row whose largest element is brought to [128, 256) end at E4M3's steps of 2^-9, half
+    of one 2^-10, for few rows in units of 1/16: an element is off by 2^-17 (few: 2^-21) of the row's largest, and a score by
+    that times sum |k|."""
     B, T, H, D = q.shape
     k, v = ref.real(layer)
     heads = k.shape[1]
     scale = D ** -0.5 if scale is None else scale
     u = torch.finfo(q.dtype).eps / 2
+    few = T * (H // heads) <= 16
+    low_p, low_q = (2.0 ** -34, 2.0 ** -21) if few else (2.0 ** -30, 2.0 ** -17)
     w = 2.0 ** -8 if q.dtype == torch.bfloat16 else 2.0 ** -11
     out, tol = torch.zeros(B, T, H, D, dtype=torch.float64), torch.zeros(B, T, H, D, dtype=torch.float64)
     for b in range(B):
@@ -100,6 +110,10 @@ def attend(ref, layer, q, lens, *, causal=True, prefix=None, q_lens=None, scale=
                 p = torch.softmax(s, 0)
                 big = ((kk[:see].abs() @ x.abs()) * abs(scale)).max().item()
                 out[b, t, h] = p @ vv[:see]
+                floor = low_q * x.abs().max().item() * kk[:see].abs().sum(1).max().item() * abs(scale)
                 spread = p @ vv[:see].abs()
-                tol[b, t, h] = u * out[b, t, h].abs() + (w * (1 + u) + 2 * ((D + 8) * 2.0 ** -23 * big + 2.0 ** -20)) * spread + 1e-30
+                blk = -(-see // ref.block)
+                faint = low_p * ref.vs[b, layer, h * heads // H, :blk].max().item() * p.max() * \
+                    values(ref.v[b, layer, h * heads // H, :see]).abs().sum(0)  # 1 / sum 2^(s_j - max s) = the largest p
+                tol[b, t, h] = u * out[b, t, h].abs() + (w * (1 + u) + 2 * ((D + 8) * 2.0 ** -23 * big + floor + 2.0 ** -20)) * spread + faint + 1e-30
     return out, tol
