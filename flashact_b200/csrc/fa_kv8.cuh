@@ -49,6 +49,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // cp.async with zero fill: copies `bytes` (0 or the full size) and zeroes the rest.
 __device__ __forceinline__ void cp_async16_zfill(void* smem_dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem_dst)), "l"(src), "r"(on ? 16 : 0)

@@ -59,13 +59,18 @@ fa_status byte_map(CUtensorMap* m, const void* base, uint64_t inner, uint64_t ro
   return FA_OK;
 }
 
-// The kernel and the splits of whole 128-key tiles.
+// The kernel and the splits of whole 128-key tiles: the number of splits with the least time by a model of measured parts (B200, us).
+// A CTA of kv8_attn_few.cu (two on an SM) pays about 4 for its start and end, and for a tile its bytes at the SM's share of the
+// memory (45 GB/s for an SM, 6.5 TB/s for all; lengths are mostly below max_len, hence 0.85). A CTA of kv8_attn_rows.cu (one on an
+// SM) pays about 10, most of it the queries' parts, and 1.9 (fp16 2.1) for a tile. Up to eight splits are a cluster (0.7);
+// more need the merge kernel (3).
 Plan make_plan(const fa_kv8* c, int tokens, int q_heads, int max_len, int sms) {
   Plan p;
   const long long all = (long long)tokens * (q_heads / c->heads);
   p.rows = all <= 8 ? 8 : all <= 16 ? 16 : 128;
   p.tiles = (int)((all + p.rows - 1) / p.rows);
-  const int chunks = std::max(1, (max_len + 127) / 128), slots = (p.rows == 128 ? 1 : 2) * sms;
+  const bool few = p.rows < 128;
+  const int chunks = std::max(1, (max_len + 127) / 128), slots = (few ? 2 : 1) * sms;
   const long long base = (long long)c->batch * c->heads * p.tiles;
   const double mb = 256e-6 * c->head_dim;  // a tile's bytes, in MB
   double best = 1e300;
@@ -73,8 +78,8 @@ Plan make_plan(const fa_kv8* c, int tokens, int q_heads, int max_len, int sms) {
   for (int n = 1; n <= 64 && n <= chunks; ++n) {
     const int each = (chunks + n - 1) / n;
     const double ctas = (double)base * n, waves = std::ceil(ctas / slots);
-    const double round = std::max(0.5, std::min(ctas, (double)slots) * mb / 6.5);
-    const double cost = waves * (3 + each * round) + (n > 8 ? 2.5 + 0.1 * n : n > 1 ? 1 : 0);
+    const double tile = few ? std::max(mb / 0.045, std::min(ctas, (double)slots) * mb * (0.85 / 6.5)) : 2.0;
+    const double cost = waves * ((few ? 4 : 10) + each * tile) + (n > 8 ? 3 + 0.1 * n : n > 1 ? 0.7 : 0);
     if (cost < best) best = cost, p.nsplit = n;
   }
   p.split_chunks = (chunks + p.nsplit - 1) / p.nsplit;

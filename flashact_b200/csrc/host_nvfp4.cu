@@ -51,13 +51,25 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   else asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// E4M3 block scale as a pair of equal 16-bit factors.
-template <bool HALF>
-__device__ __forceinline__ uint32_t factor(unsigned char s) {
-  const float f = e4m3_value(s) * Fmt<HALF>::SCALE;
-  if constexpr (HALF) return pack_f16x2(f, f);
-  const __nv_bfloat162 b = __floats2bfloat162_rn(f, f);
-  return *reinterpret_cast<const uint32_t*>(&b);
+// One or two E4M3 block scales (the low bytes of `two`), each as a pair of equal 16-bit factors.
+template <bool HALF, int N>
+__device__ __forceinline__ void factors(uint32_t two, uint32_t (&f)[N]) {
+  uint32_t v = e4m3_lo_f16x2(two);
+  if constexpr (HALF) {
+    v = mul2<true>(v, 0x58005800u);  // 2^7
+  } else {
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v));
+    const __nv_bfloat162 y = __floats2bfloat162_rn(x.x * Fmt<false>::SCALE, x.y * Fmt<false>::SCALE);
+    v = *reinterpret_cast<const uint32_t*>(&y);
+  }
+  f[0] = __byte_perm(v, 0, 0x1010);
+  if constexpr (N == 2) f[1] = __byte_perm(v, 0, 0x3232);
+}
+// A weight is read once: past L1.
+__device__ __forceinline__ uint4 ldg_stream(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
 
 struct LinArgs {
@@ -93,25 +105,30 @@ __global__ void __launch_bounds__(LW * 32) linear_kernel(const LinArgs a) {
     xon[m] = m * 8 + g < a.M;
     xp[m] = reinterpret_cast<const uint16_t*>(a.x) + (xon[m] ? (m * 8 + g) * a.ldx : 0);
   }
-  for (int p = w * 4 + t; p - t < pieces; p += LW * 4) {
+  // codes and scales of a piece, fetched one turn ahead of their use
+  uint32_t nu[RT][2][WORDS];
+  uint32_t ns[RT][2];
+  auto fetch = [&](int p) {
     const bool on = p < pieces;
-    uint32_t u[RT][2][WORDS];
-    uint32_t f[RT][2][GROUPS];
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if constexpr (PB == 16) {
-          const uint4 v = on ? __ldg(reinterpret_cast<const uint4*>(wp[r][i]) + p) : make_uint4(0, 0, 0, 0);
-          u[r][i][0] = v.x, u[r][i][1] = v.y, u[r][i][2] = v.z, u[r][i][3] = v.w;
-          const uint16_t s = on ? __ldg(reinterpret_cast<const uint16_t*>(sp[r][i]) + p) : (uint16_t)0;
-          f[r][i][0] = s & 255u, f[r][i][1] = s >> 8;
+          const uint4 v = on ? ldg_stream(reinterpret_cast<const uint4*>(wp[r][i]) + p) : make_uint4(0, 0, 0, 0);
+          nu[r][i][0] = v.x, nu[r][i][1] = v.y, nu[r][i][2] = v.z, nu[r][i][3] = v.w;
+          ns[r][i] = on ? __ldg(reinterpret_cast<const uint16_t*>(sp[r][i]) + p) : 0u;
         } else {
           const uint2 v = on ? __ldg(reinterpret_cast<const uint2*>(wp[r][i]) + p) : make_uint2(0, 0);
-          u[r][i][0] = v.x, u[r][i][1] = v.y;
-          f[r][i][0] = on ? __ldg(sp[r][i] + p) : 0u;
+          nu[r][i][0] = v.x, nu[r][i][1] = v.y;
+          ns[r][i] = on ? __ldg(sp[r][i] + p) : 0u;
         }
       }
+  };
+  fetch(w * 4 + t);
+  for (int p = w * 4 + t; p - t < pieces; p += LW * 4) {
+    const bool on = p < pieces;
+    uint32_t u[RT][2][WORDS], f[RT][2][GROUPS];
     uint4 xv[MT][WORDS];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -121,9 +138,12 @@ __global__ void __launch_bounds__(LW * 32) linear_kernel(const LinArgs a) {
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int q = 0; q < GROUPS; ++q) f[r][i][q] = factor<HALF>((unsigned char)f[r][i][q]);
+        for (int j = 0; j < WORDS; ++j) u[r][i][j] = nu[r][i][j];
+        factors<HALF>(ns[r][i], f[r][i]);
+      }
+    fetch(p + LW * 4);
 #pragma unroll
     for (int j = 0; j < WORDS; ++j) {  // eight codes: two steps of the matrix instruction
       uint32_t b[MT][4];

@@ -103,19 +103,12 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
   const int all = (top + TILE - 1) / TILE, each = a.cluster ? (all + a.nsplit - 1) / a.nsplit : a.split_chunks;
   const int t0 = split * each, nt = min(all, t0 + each) - t0;
   launch_dependents();
-  const size_t slot_id = (((size_t)b * a.heads + h) * a.tiles + tile) * a.nsplit + split;
-  if (nt <= 0) {
-    if (a.cluster) {  // nothing left for this split
-      if (tid < R) mls[tid] = make_float2(-INFINITY, 0.f);
-      cluster_join<HALF, MT>(a, osum, PITCH, reinterpret_cast<const float*>(mls), 2, split, b, h, row0, nrows, n, nq, pre);
-    } else if (split == 0) {  // no key for any of these rows: split 0 says so
-      for (int i = tid; i < nrows * a.dim; i += THREADS) {
-        const int r = i / a.dim, d = i % a.dim;
-        if (a.nsplit > 1) a.part[(slot_id * R + r) * a.dim + d] = 0.f;
-        else store16(a.out, row_at(a, b, h, row0 + r, a.ob, a.ot, a.oh) + d, 0.f, HALF);
-      }
-      if (a.nsplit > 1 && tid < nrows) a.ml[slot_id * R + tid] = make_float2(-INFINITY, 0.f);
-    }
+  const size_t first_part = ((((size_t)b * a.heads + h) * a.tiles + tile) * a.nsplit + split) * R;
+  if (nt <= 0) {  // nothing left for this split
+    if (a.nsplit > 1 && !a.cluster && split > 0) return;  // the merge knows
+    for (int i = tid; i < R * PITCH; i += THREADS) osum[i] = 0.f;
+    if (tid < R) mls[tid] = make_float2(-INFINITY, 0.f);
+    finish_rows<HALF, MT>(a, osum, PITCH, reinterpret_cast<const float*>(mls), 2, split, b, h, row0, nrows, n, nq, pre, first_part);
     return;
   }
 
@@ -347,12 +340,12 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
         l[r] += x;
         l[r + 1] += y;
         uint32_t p = pack_f16x2(x * vfac, y * vfac);
-        if (!HALF) p = round9(p);
 #pragma unroll
         for (int k = 0; k < C::PP; ++k) {
           pb[swz(k * R + r, key_lane)] = (unsigned char)(p >> 8);
           pb[swz(k * R + r + 1, key_lane)] = (unsigned char)(p >> 24);
           if (k + 1 < C::PP) p = rest8(p);
+          if (!HALF && k + 2 == C::PP) p = round_part(p);
         }
       }
       const int left = top - (t0 + i) * TILE;
@@ -383,12 +376,8 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
       float top_m = -INFINITY;
 #pragma unroll
       for (int k = 0; k < R; ++k) top_m = k == r ? m[k] : top_m;
-      if (lane == 0) {
-        mls[r] = make_float2(top_m, x);
-        if (a.nsplit > 1 && !a.cluster && r < nrows) a.ml[slot_id * R + r] = make_float2(top_m, x);
-      }
+      if (lane == 0) mls[r] = make_float2(top_m, x);
     }
-    bar_softmax();
     const float unit = vref * (1.0f / kPTop);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -404,9 +393,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
           float x = v[r] + v[R + r] * 0.125f + v[2 * R + r] * (1.0f / 64.0f);
           if (HALF) x += v[(C::PP - 1) * R + r] * (1.0f / 512.0f);
           x = ok ? x * unit : __int_as_float(0x7fffffff);  // a wait that ran out is seen in the result
-          if (a.cluster) osum[r * PITCH + d] = x;
-          else if (a.nsplit > 1) a.part[(slot_id * R + r) * a.dim + d] = x;
-          else store16(a.out, row_at(a, b, h, row0 + r, a.ob, a.ot, a.oh) + d, rowlim[r] > 0 ? x / mls[r].y : 0.f, HALF);
+          osum[r * PITCH + d] = x;
         }
       }
       __syncwarp();
@@ -415,7 +402,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
   }
   __syncthreads();
   if (w == 1) tmem_dealloc(tmem, C::COLS);
-  if (a.cluster) cluster_join<HALF, MT>(a, osum, PITCH, reinterpret_cast<const float*>(mls), 2, split, b, h, row0, nrows, n, nq, pre);
+  finish_rows<HALF, MT>(a, osum, PITCH, reinterpret_cast<const float*>(mls), 2, split, b, h, row0, nrows, n, nq, pre, first_part);
 }
 
 template <int R, bool HALF, int MT>

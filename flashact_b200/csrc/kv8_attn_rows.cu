@@ -14,8 +14,8 @@
 // P goes to tensor memory, whence the second product reads it as its first operand: shared memory then holds the queries' parts and
 // five slots of K and V tiles at head_dim 256 (with P in shared memory three, and the products waited for tiles).
 //
-// Warp 0 keeps a ring of K and V tiles (128 keys) full, warp 1 issues the products (scores of tile i + 2 before P V
-// of tile i), warps 2..9 turn scores into probabilities: a thread has one query row and half of the tile's keys, and the two
+// Warp 0 keeps a ring of K and V tiles (128 keys) full, warp 1 issues the scores' products (up to two tiles ahead),
+// warp 2 those of P and V, warps 4..11 turn scores into probabilities: a thread has one query row and half of the tile's keys, and the two
 // threads of a row exchange their maxima, those of tile i + 1 while they write P of tile i. The running maximum moves only where it grew by more than 2^1, the only
 // case that touches O.
 #include "kv8_tc.cuh"
@@ -25,7 +25,7 @@ namespace {
 using namespace fa;
 using namespace fa::kv8;
 
-constexpr int THREADS = 320, ROWS = 128;
+constexpr int THREADS = 384, ROWS = 128, SOFT = 4;  // SOFT: first softmax warp
 constexpr float kPTop = 16384.0f;  // p = 1; with a maximum that lags by up to kLag, 2^15 (E5M2 ends at 57344)
 constexpr float kLag = 1.0f;
 
@@ -80,19 +80,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int all = (top + TILE - 1) / TILE, each = a.cluster ? (all + a.nsplit - 1) / a.nsplit : a.split_chunks;
   const int t0 = split * each, nt = min(all, t0 + each) - t0;
   launch_dependents();
-  const size_t slot_id = (((size_t)b * a.heads + h) * a.tiles + tile) * a.nsplit + split;
-  if (nt <= 0) {
-    if (a.cluster) {  // nothing left for this split
-      if (tid < ROWS) *reinterpret_cast<float2*>(osum + tid * PITCH + MT * 128) = make_float2(-INFINITY, 0.f);
-      cluster_join<HALF, MT>(a, osum, PITCH, osum + MT * 128, PITCH, split, b, h, row0, nrows, n, nq, pre);
-    } else if (split == 0) {  // no key for any of these rows: split 0 says so
-      for (int i = tid; i < nrows * a.dim; i += THREADS) {
-        const int r = i / a.dim, d = i % a.dim;
-        if (a.nsplit > 1) a.part[(slot_id * ROWS + r) * a.dim + d] = 0.f;
-        else store16(a.out, row_at(a, b, h, row0 + r, a.ob, a.ot, a.oh) + d, 0.f, HALF);
-      }
-      if (a.nsplit > 1 && tid < nrows) a.ml[slot_id * ROWS + tid] = make_float2(-INFINITY, 0.f);
-    }
+  const size_t first_part = ((((size_t)b * a.heads + h) * a.tiles + tile) * a.nsplit + split) * ROWS;
+  if (nt <= 0) {  // nothing left for this split
+    if (a.nsplit > 1 && !a.cluster && split > 0) return;  // the merge knows
+    for (int i = tid; i < ROWS * PITCH; i += THREADS) osum[i] = i % PITCH == MT * 128 ? -INFINITY : 0.f;
+    finish_rows<HALF, MT>(a, osum, PITCH, osum + MT * 128, PITCH, split, b, h, row0, nrows, n, nq, pre, first_part);
     return;
   }
 
@@ -115,19 +107,19 @@ __global__ void __launch_bounds__(THREADS, 1)
     tmem_relinquish();
   }
   float vref = 0.f;  // largest V scale of the split
-  if (w >= 2) {
+  if (w >= SOFT) {
     const int kend = min(top, (t0 + nt) * TILE);
-    for (int i = ((t0 * TILE) >> a.block_log2) + tid - 64; (i << a.block_log2) < kend; i += 256) vref = fmaxf(vref, vs[i]);
+    for (int i = ((t0 * TILE) >> a.block_log2) + tid - SOFT * 32; (i << a.block_log2) < kend; i += 256) vref = fmaxf(vref, vs[i]);
     // queries: power-of-two row scales and E4M3 parts; rows behind the last are zero
     constexpr int LANES = MT * 16, PER = 32 / LANES, N = 16 / PER;  // lanes of a row, rows at a time, such groups of the warp's 16 rows
     const int l8 = (lane % LANES) * 8;                              // this lane's dims, l8 .. + 7
     auto source = [&](int j) {
-      const int r = row0 + (w - 2) * 16 + j * PER + lane / LANES;
+      const int r = row0 + (w - SOFT) * 16 + j * PER + lane / LANES;
       return token_of(a, r) < a.mask.tokens && l8 < a.dim
                  ? reinterpret_cast<const uint16_t*>(a.q) + row_at(a, b, h, r, a.qb, a.qt, a.qh) + l8 : nullptr;
     };
     auto split = [&](int j, uint4 q) {
-      const int r = (w - 2) * 16 + j * PER + lane / LANES;
+      const int r = (w - SOFT) * 16 + j * PER + lane / LANES;
       const float2 x0 = pair_f32<HALF>(q.x), x1 = pair_f32<HALF>(q.y), x2 = pair_f32<HALF>(q.z), x3 = pair_f32<HALF>(q.w);
       float m = fmaxf(fmaxf(fmaxf(fabsf(x0.x), fabsf(x0.y)), fmaxf(fabsf(x1.x), fabsf(x1.y))),
                       fmaxf(fmaxf(fabsf(x2.x), fabsf(x2.y)), fmaxf(fabsf(x3.x), fabsf(x3.y))));
@@ -143,31 +135,28 @@ __global__ void __launch_bounds__(THREADS, 1)
         *reinterpret_cast<uint2*>(qs + (p * MT + (l8 >> 7)) * 16384 + swz(r, l8 & 127)) = make_uint2(e[p], v);
       });
     };
-    if (a.q_wide) {  // all loads on their way first
-      uint4 q[N];
+    auto load = [&](int j) {
+      const uint16_t* p = j < N ? source(j) : nullptr;
+      if (!p) return make_uint4(0, 0, 0, 0);
+      if (a.q_wide) return __ldg(reinterpret_cast<const uint4*>(p));
+      uint32_t u[4];
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const uint16_t* p = source(j);
-        q[j] = p ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int j = 0; j < N; ++j) split(j, q[j]);
-    } else {
+      for (int k = 0; k < 4; ++k) u[k] = (uint32_t)__ldg(p + 2 * k) | ((uint32_t)__ldg(p + 2 * k + 1) << 16);
+      return make_uint4(u[0], u[1], u[2], u[3]);
+    };
+    // two rows (or pairs of rows) a turn, the next two on their way; rolled, since straight code would be fetched cold
+    uint4 q0 = load(0), q1 = load(1);
 #pragma unroll 1
-      for (int j = 0; j < N; ++j) {
-        const uint16_t* p = source(j);
-        uint32_t u[4] = {0, 0, 0, 0};
-        if (p) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) u[k] = (uint32_t)__ldg(p + 2 * k) | ((uint32_t)__ldg(p + 2 * k + 1) << 16);
-        }
-        __syncwarp();
-        split(j, make_uint4(u[0], u[1], u[2], u[3]));
-      }
+    for (int j = 0; j < N; j += 2) {
+      const uint4 n0 = load(j + 2), n1 = load(j + 3);
+      __syncwarp();
+      split(j, q0);
+      split(j + 1, q1);
+      q0 = n0, q1 = n1;
     }
     fence_proxy_async_shared();
     vref = warp_max(vref);
-    if (lane == 0) red[w - 2] = vref;
+    if (lane == 0) red[w - SOFT] = vref;
   }
   tc_fence_before();
   __syncthreads();
@@ -179,7 +168,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncwarp();
   } else if (w == 1) {
     const int steps = a.dim / 32;
-    const uint32_t ids = idesc_f8(TILE, false, false), idp = idesc_f8(a.dim, true, false);
+    const uint32_t ids = idesc_f8(TILE, false, false);
     const uint32_t qa = desc_lo(qs);
     bool ok = true;
     auto scores = [&](int i) {
@@ -198,13 +187,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_commit_elect(sfull);
       tc_commit_elect(empty + slot);
     };
-    scores(0);
-    if (nt > 1 && ok) scores(1);
-    for (int i = 0; i < nt && ok; ++i) {
-      if (i + 2 < nt) scores(i + 2);  // scores i + 1 have been read by then, before P of tile i is there
-      ok = ok && mbar_wait(pfull, i & 1, err, ERR_P);
+    for (int i = 0; i < nt && ok; ++i) scores(i);
+  } else if (w == 2) {  // a warp of its own: a product is issued in about 100 cycles beside the softmax, and takes 64 or 128
+    const uint32_t idp = idesc_f8(a.dim, true, false);
+    bool ok = true;
+    for (int i = 0; i < nt; ++i) {
       const int pos = pos_v<2>(i, nt), slot = pos % C::SLOTS;
       ok = ok && mbar_wait(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
+      ok = ok && mbar_wait(pfull, i & 1, err, ERR_P);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -216,8 +206,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_commit_elect(pvdone);
       tc_commit_elect(empty + slot);
     }
-  } else {
-    const int sw = w - 2, half = sw >> 2, quad = w & 3, row = quad * 32 + lane, st = tid - 64;
+  } else if (w >= SOFT) {
+    const int half = (w - SOFT) >> 2, quad = w & 3, row = quad * 32 + lane, st = tid - SOFT * 32;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
 #pragma unroll
     for (int i = 0; i < 8; ++i) vref = fmaxf(vref, red[i]);
@@ -268,10 +258,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        float g = fmaxf(s[16 * j], s[16 * j + 1]);
+        float g = s[16 * j];
 #pragma unroll
-        for (int c = 2; c < 16; c += 2) g = fmaxf(fmaxf(g, s[16 * j + c]), s[16 * j + c + 1]);
-        mx = fmaxf(mx, g * f[j]);
+        for (int c = 1; c < 15; c += 2) g = max3(g, s[16 * j + c], s[16 * j + c + 1]);
+        mx = fmaxf(mx, fmaxf(g, s[16 * j + 15]) * f[j]);
       }
       half_max[(i & 1) * 2 * ROWS + half * ROWS + row] = mx;
       __syncwarp();
@@ -309,21 +299,29 @@ __global__ void __launch_bounds__(THREADS, 1)
       const float base = m == -INFINITY ? 0.f : m;
       uint32_t e[C::PP][16];  // all of P before the wait for its place, which the product of the tile before still reads
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 4; ++j) {
+        // p vs / vref 2^14 straight from the exponent; the sum of p is that of a group over its factor. A factor below 2^-40 counts as
+        // that: such a P is 0 in f16 either way.
+        const float v = vf[j] < 9.094947e-13f ? 9.094947e-13f : vf[j], lv = log2_approx(v);
+        const uint64_t ff = pack2(f[j], f[j]), cc = pack2(lv - base, lv - base);
+        uint64_t g = 0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const float* x = s + 16 * j + 4 * c;
-          const float x0 = exp2_approx(fmaf(x[0], f[j], -base)), x1 = exp2_approx(fmaf(x[1], f[j], -base));
-          const float x2 = exp2_approx(fmaf(x[2], f[j], -base)), x3 = exp2_approx(fmaf(x[3], f[j], -base));
-          l += (x0 + x1) + (x2 + x3);
-          uint32_t p = pack_f16x2(x0 * vf[j], x1 * vf[j]), q = pack_f16x2(x2 * vf[j], x3 * vf[j]);
-          if (!HALF) p = round9(p), q = round9(q);
+          const float2 y = unpack2(fma2(pack2(x[0], x[1]), ff, cc)), z = unpack2(fma2(pack2(x[2], x[3]), ff, cc));
+          const float x0 = exp2_approx(y.x), x1 = exp2_approx(y.y), x2 = exp2_approx(z.x), x3 = exp2_approx(z.y);
+          g = add2(g, add2(pack2(x0, x1), pack2(x2, x3)));
+          uint32_t p = pack_f16x2(x0, x1), q = pack_f16x2(x2, x3);
 #pragma unroll
           for (int k = 0; k < C::PP; ++k) {
+            if (!HALF && k + 1 == C::PP) p = round_part(p), q = round_part(q);
             e[k][4 * j + c] = __byte_perm(p, q, 0x7531);  // the upper bytes
             if (k + 1 < C::PP) p = rest1(p), q = rest1(q);
           }
         }
+        const float2 sum = unpack2(g);
+        l += (sum.x + sum.y) * exp2_approx(-lv);
+      }
       if (i + 1 < nt) fetch(i + 1);
       if (!ok) break;
       if (i > 0) {
@@ -354,52 +352,24 @@ __global__ void __launch_bounds__(THREADS, 1)
     sums[half * ROWS + row] = l;
     bar_softmax();
     l = sums[row] + sums[ROWS + row];
-    if (half == 0) {
-      if (a.cluster) *reinterpret_cast<float2*>(osum + row * PITCH + MT * 128) = make_float2(m, l);
-      else if (a.nsplit > 1 && row < nrows) a.ml[slot_id * ROWS + row] = make_float2(m, l);
-    }
-    const float unit = vref * (1.0f / kPTop);
-    const float norm = !ok ? __int_as_float(0x7fffffff)  // a wait that ran out is seen in the result
-                           : a.nsplit > 1 ? unit : lim > 0 ? unit / l : 0.f;
-    uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + row_at(a, b, h, row0 + row, a.ob, a.ot, a.oh);
-#pragma unroll 2
-    for (int c = half * 16; c < a.dim; c += 32) {
-      float v[16];
+    if (half == 0) *reinterpret_cast<float2*>(osum + row * PITCH + MT * 128) = make_float2(m, l);
+    const float norm = ok ? vref * (1.0f / kPTop) : __int_as_float(0x7fffffff);  // a wait that ran out is seen in the result
+#pragma unroll 1
+    for (int c = half * 32; c < a.dim; c += 64) {
+      float v[32];
       tmem_ld16(tmem_o + lanes + c, v);
+      tmem_ld16(tmem_o + lanes + c + 16, v + 16);
       tc_wait_ld();
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = ok && lim <= 0 ? 0.f : v[j] * norm;
-      if (row >= nrows) {
-        // not a row of the call
-      } else if (a.nsplit > 1) {
-        float4* p = reinterpret_cast<float4*>(a.cluster ? osum + row * PITCH + c : a.part + (slot_id * ROWS + row) * a.dim + c);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-      } else {
-        uint32_t u[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const __nv_bfloat162 bv = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-          u[j] = HALF ? pack_f16x2(v[2 * j], v[2 * j + 1]) : *reinterpret_cast<const uint32_t*>(&bv);
-        }
-        if ((reinterpret_cast<uintptr_t>(out + c) & 15) == 0) {
-          reinterpret_cast<uint4*>(out + c)[0] = make_uint4(u[0], u[1], u[2], u[3]);
-          reinterpret_cast<uint4*>(out + c)[1] = make_uint4(u[4], u[5], u[6], u[7]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            out[c + 2 * j] = (uint16_t)u[j];
-            out[c + 2 * j + 1] = (uint16_t)(u[j] >> 16);
-          }
-        }
-      }
-      __syncwarp();
+      for (int j = 0; j < 8; ++j)
+        *reinterpret_cast<float4*>(osum + row * PITCH + c + 4 * j) =
+            make_float4(v[4 * j] * norm, v[4 * j + 1] * norm, v[4 * j + 2] * norm, v[4 * j + 3] * norm);
     }
     tc_fence_before();
   }
   __syncthreads();
   if (w == 1) tmem_dealloc(tmem_o, 512);
-  if (a.cluster) cluster_join<HALF, MT>(a, osum, PITCH, osum + MT * 128, PITCH, split, b, h, row0, nrows, n, nq, pre);
+  finish_rows<HALF, MT>(a, osum, PITCH, osum + MT * 128, PITCH, split, b, h, row0, nrows, n, nq, pre, first_part);
 }
 
 template <bool HALF, int MT>

@@ -46,6 +46,32 @@ __host__ __device__ constexpr uint32_t idesc_f8(int N, bool a_e5m2, bool b_e5m2)
   return (1u << 4) | ((a_e5m2 ? 1u : 0u) << 7) | ((b_e5m2 ? 1u : 0u) << 10) | ((uint32_t)(N >> 3) << 17) |
          ((uint32_t)(128 >> 4) << 24);
 }
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
 __device__ __forceinline__ float warp_max(float x) {
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
@@ -57,9 +83,9 @@ __device__ __forceinline__ uint32_t f32x2_e4m3x2(float lo, float hi) {
   return r;
 }
 // E5M2 is f16's upper byte: cutting a non-negative f16 there leaves its first three significant bits, and what was cut off is
-// again an f16. Three such parts hold nine bits, four all eleven. P is rounded to nine beforehand (no carry leaves a
-// half, p being at most 2^15; a NaN is lost here, but its row's sum has it too).
-__device__ __forceinline__ uint32_t round9(uint32_t p) { return (p + 0x00020002u) & 0xfffcfffcu; }
+// again an f16. Four such parts hold all its eleven bits; of three, the last is rounded instead of cut (p is at most 2^15, so
+// that no carry leaves a half).
+__device__ __forceinline__ uint32_t round_part(uint32_t p) { return p + 0x00800080u; }
 __device__ __forceinline__ uint32_t rest1(uint32_t p) {
   const uint32_t v = p & 0xff00ff00u;
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&p), *reinterpret_cast<const __half2*>(&v));
@@ -140,11 +166,22 @@ __device__ __forceinline__ void store16x4(uint16_t* p, float x, float y, float z
     p[2] = (uint16_t)u.y, p[3] = (uint16_t)(u.y >> 16);
   }
 }
-// Joins the splits' sums `o` [rows][pitch] (relative to their maxima) with their maxima and sums `ml`, in split order; the
-// CTAs of the cluster share the output, a warp takes 128 dims of a row. All threads of all its CTAs come here.
+// The end of a tile of rows: sums `o` [rows][pitch] relative to their maxima, and (maximum, sum) `ml`, in shared memory.
+// More than eight splits leave both for the merge kernel. Otherwise the splits, a cluster (or the only CTA), are joined in
+// split order, its CTAs sharing the output; a warp takes 128 dims of a row. All threads of all the CTAs come here.
 template <bool HALF, int MT>
-__device__ __forceinline__ void cluster_join(const AttnArgs& a, const float* o, int pitch, const float* ml, int ml_pitch,
-                                             int rank, int b, int h, int row0, int nrows, int n, int nq, int pre) {
+__device__ __forceinline__ void finish_rows(const AttnArgs& a, const float* o, int pitch, const float* ml, int ml_pitch, int rank,
+                                            int b, int h, int row0, int nrows, int n, int nq, int pre, size_t first_part) {
+  if (a.nsplit > 1 && !a.cluster) {
+    __syncthreads();
+    for (int u = threadIdx.x >> 5; u < nrows * MT; u += blockDim.x >> 5) {
+      const int r = u / MT, d = (u % MT) * 128 + (threadIdx.x & 31) * 4;
+      if (d < a.dim)
+        *reinterpret_cast<float4*>(a.part + (first_part + r) * a.dim + d) = *reinterpret_cast<const float4*>(o + r * pitch + d);
+      if (d == 0) a.ml[first_part + r] = *reinterpret_cast<const float2*>(ml + r * ml_pitch);
+    }
+    return;
+  }
   cluster_sync();
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   for (int u = rank * warps + (threadIdx.x >> 5); u < nrows * MT; u += a.nsplit * warps) {

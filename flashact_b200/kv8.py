@@ -11,6 +11,14 @@ import torch
 from . import _capi as C
 from .pi05 import _DT
 
+_byref = ctypes.byref
+_current_device = torch.cuda.current_device
+
+
+def _current_stream(index):
+    """The raw current stream of a device: what torch.cuda.current_stream(index).cuda_stream gives, without the object."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
 
 def _bad(msg):
     return C.FlashActError(C.FA_ERR_INVALID, msg)
@@ -57,7 +65,7 @@ class Kv8Cache:
             if tuple(t.shape) != shape or t.dtype != dt or not t.is_contiguous() or t.device != k.device or not t.is_cuda:
                 raise _bad(f"'{name}' must be a contiguous {dt} CUDA tensor of shape {shape} on k's device, "
                            f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-        self.k, self.v, self.k_scale, self.v_scale, self.lens = k, v, k_scale, v_scale, lens
+        self.k, self.v, self.k_scale, self.v_scale, self._lens_tensor = k, v, k_scale, v_scale, lens
         self.batch, self.layers, self.heads, self.capacity, self.head_dim = b, layers, heads, cap, d
         self.block = cap // blocks
         self.device = k.device
@@ -66,34 +74,41 @@ class Kv8Cache:
                           self.block)
         self._ref = ctypes.byref(self._c)
         self._ws = {}  # workspace bytes of the shapes asked for
+        self._index, self._lens, self._scale = self.device.index, lens.data_ptr(), d ** -0.5
+        self._append, self._attention = self.lib.fa_kv8_append, self.lib.fa_kv8_attention
+
+    @property
+    def lens(self):
+        return self._lens_tensor
+
+    @lens.setter
+    def lens(self, t):
+        self._lens, self._lens_tensor = self._ints("lens", t), t
 
     def _check(self, st):
         if st != C.FA_OK:
             C.check(self.lib, None, st)
 
-    def _on(self, stream, fn):
-        """Runs fn(raw stream) with the cache's device current and, for a stream given, on it."""
-        if stream is not None:
-            with torch.cuda.stream(stream):
-                return fn(stream.cuda_stream)
-        if torch.cuda.current_device() != self.device.index:
-            with torch.cuda.device(self.device):
-                return fn(torch.cuda.current_stream(self.device).cuda_stream)
-        return fn(torch.cuda.current_stream(self.device).cuda_stream)
+    def _elsewhere(self, stream):
+        """The context in which a call on `stream`, or on a cache of another device than the current one, is made."""
+        return torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.device)
 
     def _rows(self, name, t, heads):
-        if t.dim() != 4 or t.shape[0] != self.batch or t.shape[2] != heads or t.shape[3] != self.head_dim:
-            raise _bad(f"'{name}' must be [{self.batch}][tokens][{heads}][{self.head_dim}], got {tuple(t.shape)}")
+        shape = t.shape
+        if len(shape) != 4 or shape[0] != self.batch or shape[2] != heads or shape[3] != self.head_dim:
+            raise _bad(f"'{name}' must be [{self.batch}][tokens][{heads}][{self.head_dim}], got {tuple(shape)}")
         if t.device != self.device:
             raise _bad(f"'{name}' is on {t.device}, the cache on {self.device}")
-        if t.stride(3) != 1:
+        st = t.stride()
+        if st[3] != 1:
             t = t.contiguous()
-        return t, C.FaRows(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+            st = t.stride()
+        return t, C.FaRows(t.data_ptr(), st[0], st[1], st[2])
 
     def _ints(self, name, t):
         if t is None:
             return None
-        if t.dtype != torch.int32 or tuple(t.shape) != (self.batch,) or not t.is_contiguous() or t.device != self.device:
+        if t.dtype != torch.int32 or t.shape != self._lens_tensor.shape or not t.is_contiguous() or t.device != self.device:
             raise _bad(f"'{name}' must be a contiguous int32 tensor [{self.batch}] on {self.device}")
         return t.data_ptr()
 
@@ -101,17 +116,20 @@ class Kv8Cache:
                start: torch.Tensor | None = None, stream=None):
         """Quantises k, v [batch][tokens][heads][head_dim] (fp32, bf16 or fp16, any strides) into `layer` behind `start`
         (default: lens). count (int32 [batch]) gives each observation's number of real rows in a padded batch."""
-        if k.dtype not in _DT or v.dtype != k.dtype:
+        if stream is not None or _current_device() != self._index:
+            with self._elsewhere(stream):
+                return self.append(layer, k, v, count=count, start=start)
+        dt = _DT.get(k.dtype)
+        if dt is None or v.dtype != k.dtype:
             raise _bad(f"k and v must share fp32, bf16 or fp16, got {k.dtype} and {v.dtype}")
-        if k.dim() == 4 and v.dim() == 4 and k.shape[1] != v.shape[1]:
-            raise _bad(f"{k.shape[1]} rows of k and {v.shape[1]} of v")
-
-        def call(s):
-            (kt, kr), (vt, vr) = self._rows("k", k, self.heads), self._rows("v", v, self.heads)
-            self._check(self.lib.fa_kv8_append(self._ref, layer, k.shape[1], ctypes.byref(kr), ctypes.byref(vr), _DT[k.dtype],
-                                               self._ints("start", self.lens if start is None else start),
-                                               self._ints("count", count), s))
-        self._on(stream, call)
+        k, kr = self._rows("k", k, self.heads)
+        v, vr = self._rows("v", v, self.heads)
+        rows = k.shape[1]
+        if v.shape[1] != rows:
+            raise _bad(f"{rows} rows of k and {v.shape[1]} of v")
+        self._check(self._append(self._ref, layer, rows, _byref(kr), _byref(vr), dt,
+                                 self._lens if start is None else self._ints("start", start), self._ints("count", count),
+                                 _current_stream(self._index)))
 
     def advance(self, n):
         """lens += n (a number, or a tensor [batch]) after every layer has appended."""
@@ -125,43 +143,46 @@ class Kv8Cache:
         them. causal: token i of an observation's q_lens (default: tokens) stands at lens - q_lens + i and sees the
         keys up to there, and all below prefix; not causal: every key. max_len: an upper bound of lens that the host knows
         (default: the capacity). Rows of `out` behind q_lens are left as they were (zero in a new tensor)."""
-        if q.dtype not in _DT or q.dim() != 4:
-            raise _bad(f"q must be a bf16 or fp16 tensor of four dimensions, got {q.dtype} {tuple(q.shape)}")
-        b, tokens, q_heads, d = q.shape
-
-        def call(s):
-            qt, qr = self._rows("q", q, q_heads)
-            o = out
-            if o is None:
-                o = (torch.empty if q_lens is None else torch.zeros)((b, tokens, q_heads, d), dtype=q.dtype, device=q.device)
-            elif o.shape != q.shape or o.dtype != q.dtype or o.device != q.device or (o.numel() and o.stride(3) != 1):
-                raise _bad(f"'out' must be like q ({q.dtype} {tuple(q.shape)}) with a contiguous last dimension")
-            orow = C.FaRows(o.data_ptr(), o.stride(0), o.stride(1), o.stride(2))
-            key = (tokens, q_heads, max_len)
-            need = self._ws.get(key)
-            if need is None:
-                n = ctypes.c_size_t()
-                self._check(self.lib.fa_kv8_attention_workspace(self._ref, tokens, q_heads, max_len, ctypes.byref(n)))
-                need = self._ws[key] = n.value
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-            self._check(self.lib.fa_kv8_attention(
-                self._ref, layer, tokens, q_heads, ctypes.byref(qr), _DT[q.dtype], self._ints("lens", self.lens if lens is None else lens),
-                self._ints("q_lens", q_lens), self._ints("prefix", prefix), int(causal), d ** -0.5 if scale is None else scale,
-                max_len, ctypes.byref(orow), ws.data_ptr() if need else None, need, s))
-            return o
-        return self._on(stream, call)
+        if stream is not None or _current_device() != self._index:
+            with self._elsewhere(stream):
+                return self.attend(layer, q, scale=scale, causal=causal, prefix=prefix, q_lens=q_lens, lens=lens,
+                                   max_len=max_len, out=out)
+        dt, shape = _DT.get(q.dtype), q.shape
+        if dt is None or len(shape) != 4:
+            raise _bad(f"q must be a bf16 or fp16 tensor of four dimensions, got {q.dtype} {tuple(shape)}")
+        tokens, q_heads = shape[1], shape[2]
+        q, qr = self._rows("q", q, q_heads)
+        if out is None:
+            out = torch.empty(shape, dtype=q.dtype, device=self.device)
+            if q_lens is not None:
+                out.zero_()
+        elif out.shape != shape or out.dtype != q.dtype or out.device != self.device or (out.numel() and out.stride(3) != 1):
+            raise _bad(f"'out' must be like q ({q.dtype} {tuple(shape)}) with a contiguous last dimension")
+        st = out.stride()
+        orow = C.FaRows(out.data_ptr(), st[0], st[1], st[2])
+        need = self._ws.get((tokens, q_heads, max_len))
+        if need is None:
+            n = ctypes.c_size_t()
+            self._check(self.lib.fa_kv8_attention_workspace(self._ref, tokens, q_heads, max_len, _byref(n)))
+            need = self._ws[tokens, q_heads, max_len] = n.value
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        self._check(self._attention(
+            self._ref, layer, tokens, q_heads, _byref(qr), dt, self._lens if lens is None else self._ints("lens", lens),
+            self._ints("q_lens", q_lens), self._ints("prefix", prefix), causal, self._scale if scale is None else scale, max_len,
+            _byref(orow), ws.data_ptr() if need else None, need, _current_stream(self._index)))
+        return out
 
     def read(self, rows: int, *, dtype=torch.bfloat16, lens: torch.Tensor | None = None, stream=None):
         """(K, V) as values [batch][layers][rows][heads * head_dim], zero at and behind each length."""
+        if stream is not None or _current_device() != self._index:
+            with self._elsewhere(stream):
+                return self.read(rows, dtype=dtype, lens=lens)
         if dtype not in _DT:
             raise _bad(f"values are fp32, bf16 or fp16, not {dtype}")
         if rows < 0:
             raise _bad(f"rows={rows}")
-
-        def call(s):
-            k, v = (torch.empty(self.batch, self.layers, rows, self.heads * self.head_dim, dtype=dtype, device=self.device)
-                    for _ in range(2))
-            self._check(self.lib.fa_kv8_read(self._ref, self._ints("lens", self.lens if lens is None else lens), rows,
-                                             k.data_ptr(), v.data_ptr(), _DT[dtype], s))
-            return k, v
-        return self._on(stream, call)
+        shape = (self.batch, self.layers, rows, self.heads * self.head_dim)
+        k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
+        self._check(self.lib.fa_kv8_read(self._ref, self._lens if lens is None else self._ints("lens", lens), rows, k.data_ptr(),
+                                         v.data_ptr(), _DT[dtype], _current_stream(self._index)))
+        return k, v

@@ -63,36 +63,36 @@ def nvfp4_linear(x: torch.Tensor, packed: torch.Tensor, block_scale: torch.Tenso
     """x W^T * tensor_scale (+ bias) for x [..., K] (bf16 or fp16) of up to 16 rows and one layer's matrix as
     quantize_nvfp4 gives it: packed uint8 [N, K/2], block_scale uint8 [N, K/16], tensor_scale fp32 of one element;
     bias fp32 [N]. Returns [..., N] in x's type."""
-    lib = C.load_library()
-    if x.dim() < 1 or x.dtype not in _DT or not x.is_cuda:
+    dt, shape, dev = _DT.get(x.dtype), x.shape, x.device
+    if dt is None or not shape or not x.is_cuda:
         raise C.FlashActError(C.FA_ERR_INVALID, "x must be a CUDA tensor [..., K]")
-    K, dev = x.shape[-1], x.device
-    N = packed.shape[0] if packed.dim() == 2 else 0
-    for name, t, shape, dt in (("packed", packed, (N, K // 2), torch.uint8), ("block_scale", block_scale, (N, K // 16), torch.uint8),
-                               ("tensor_scale", tensor_scale, None, torch.float32), ("bias", bias, (N,), torch.float32)):
-        if t is None and name == "bias":
-            continue
-        if (t.numel() != 1 if shape is None else t.shape != shape) or t.dtype != dt or t.device != dev or not t.is_contiguous():
-            raise C.FlashActError(C.FA_ERR_INVALID, f"'{name}' must be a contiguous {dt} tensor {shape or '(one element)'} on "
-                                                    f"{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    shape = (*x.shape[:-1], N)
-    if out is not None and (out.shape != shape or out.dtype != x.dtype or out.device != dev or not out.is_contiguous()):
+    if stream is not None or torch.cuda.current_device() != dev.index:
+        with torch.cuda.stream(stream) if stream is not None else torch.cuda.device(dev):
+            return nvfp4_linear(x, packed, block_scale, tensor_scale, bias=bias, out=out)
+    K, pshape = shape[-1], packed.shape
+    N = pshape[0] if len(pshape) == 2 else 0
+    _operand("packed", packed, (N, K // 2), torch.uint8, dev)
+    _operand("block_scale", block_scale, (N, K // 16), torch.uint8, dev)
+    _operand("tensor_scale", tensor_scale, None, torch.float32, dev)
+    if bias is not None:
+        _operand("bias", bias, (N,), torch.float32, dev)
+    shape = (*shape[:-1], N)
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=dev)
+    elif out.shape != shape or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
         raise C.FlashActError(C.FA_ERR_INVALID, f"'out' must be a contiguous {x.dtype} tensor {tuple(shape)} on {dev}")
+    if not x.is_contiguous():
+        x = x.contiguous()
+    if x.data_ptr() % 16:
+        x = x.clone()
+    lib = C.load_library()
+    _check(lib, lib.fa_nvfp4_linear(x.data_ptr(), dt, x.numel() // K if K else 0, K, K, packed.data_ptr(), block_scale.data_ptr(),
+                                    tensor_scale.data_ptr(), None if bias is None else bias.data_ptr(), N, out.data_ptr(), N,
+                                    torch._C._cuda_getCurrentRawStream(dev.index)))
+    return out
 
-    def call(s):
-        xc = x.contiguous()
-        if xc.data_ptr() % 16:
-            xc = xc.clone()
-        y = torch.empty(shape, dtype=x.dtype, device=dev) if out is None else out
-        _check(lib, lib.fa_nvfp4_linear(xc.data_ptr(), _DT[x.dtype], xc.numel() // K if K else 0, K, K, packed.data_ptr(),
-                                        block_scale.data_ptr(), tensor_scale.data_ptr(),
-                                        None if bias is None else bias.data_ptr(), N, y.data_ptr(), N, s))
-        return y
 
-    if stream is not None:
-        with torch.cuda.stream(stream):
-            return call(stream.cuda_stream)
-    if torch.cuda.current_device() != dev.index:
-        with torch.cuda.device(dev):
-            return call(torch.cuda.current_stream(dev).cuda_stream)
-    return call(torch.cuda.current_stream(dev).cuda_stream)
+def _operand(name, t, shape, dtype, dev):
+    if (t.numel() != 1 if shape is None else t.shape != shape) or t.dtype != dtype or t.device != dev or not t.is_contiguous():
+        raise C.FlashActError(C.FA_ERR_INVALID, f"'{name}' must be a contiguous {dtype} tensor {shape or '(one element)'} on {dev}, "
+                                                f"got {t.dtype} {tuple(t.shape)} on {t.device}")
