@@ -222,7 +222,7 @@ struct ReadArgs {
   const float *ks, *vs;
   const int* lens;
   void *ok, *ov;
-  int rows, layers, heads, D, cap, block;
+  int rows, layers, heads, D, cap, block, block_log2;
 };
 
 // Two codes (the low 16 bits) times a scale.
@@ -232,7 +232,7 @@ __device__ __forceinline__ float2 values2(uint32_t two, float s) {
   return make_float2(v.x * s, v.y * s);
 }
 template <class T>
-__device__ __forceinline__ void store8(T* p, const float2 (&v)[4]) {
+__device__ __forceinline__ void store8(T* p, const float2* v) {
   if constexpr (sizeof(T) == 4) {
     reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
     reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
@@ -252,11 +252,13 @@ __device__ __forceinline__ void store8(T* p, const float2 (&v)[4]) {
 }
 
 // One CTA per 64 tokens of a (observation, layer, head): K and V back as values [batch][layers][rows][heads * D]; rows at and behind
-// the observation's length are zero. V is turned around in registers: a thread reads four tokens of eight dims (a warp
-// 64 bytes of a transposed row) and writes eight dims of four tokens.
+// the observation's length are zero. V is turned around through shared memory, words of four tokens at an index that is
+// mixed with the dim so that a warp finds its words in different banks, and its rows are written whole: in pieces of 32 bytes they took
+// a half longer.
 constexpr int RT = 64;
 template <class T>
 __global__ void __launch_bounds__(256) read_kernel(ReadArgs a) {
+  extern __shared__ uint32_t words[];  // [D][RT / 4], word t of row d at t ^ (d / 8 % 16)
   const int bl = blockIdx.z, h = blockIdx.y, r0 = blockIdx.x * RT, tid = threadIdx.x;
   const int len = min(min(max(a.lens[bl / a.layers], 0), a.cap), a.rows);
   const size_t hd = (size_t)bl * a.heads + h;
@@ -265,28 +267,37 @@ __global__ void __launch_bounds__(256) read_kernel(ReadArgs a) {
   const size_t width = (size_t)a.heads * a.D;
   T* ok = reinterpret_cast<T*>(a.ok) + (size_t)bl * a.rows * width + h * a.D;
   T* ov = reinterpret_cast<T*>(a.ov) + (size_t)bl * a.rows * width + h * a.D;
-  const int D8 = a.D / 8, n = min(RT, a.rows - r0);
+  // K: a thread has 16 dims of a row, then of the row `step` below; no division in the loop
+  const int D16 = a.D / 16, step = 256 / D16, d16 = tid % D16 * 16, end = min(RT, a.rows - r0);
 #pragma unroll 2
-  for (int i = tid; i < n * D8; i += 256) {
-    const int r = r0 + i / D8, d = (i % D8) * 8;
-    float2 x[4] = {};
-    if (r < len) {
-      const uint2 c = __ldg(reinterpret_cast<const uint2*>(k + (size_t)r * a.D + d));
-      const float s = __ldg(ks + r / a.block);
+  for (int r = tid / D16; r < end && tid < step * D16; r += step) {
+    float2 x[8] = {};
+    if (r0 + r < len) {
+      const uint4 c = __ldg(reinterpret_cast<const uint4*>(k + (size_t)(r0 + r) * a.D + d16));
+      const float s = __ldg(ks + ((r0 + r) >> a.block_log2));
       x[0] = values2(c.x, s), x[1] = values2(c.x >> 16, s), x[2] = values2(c.y, s), x[3] = values2(c.y >> 16, s);
+      x[4] = values2(c.z, s), x[5] = values2(c.z >> 16, s), x[6] = values2(c.w, s), x[7] = values2(c.w >> 16, s);
     }
-    store8<T>(ok + (size_t)r * width + d, x);
+    T* o = ok + (size_t)(r0 + r) * width + d16;
+    store8<T>(o, x);
+    store8<T>(o + 8, x + 4);
   }
+  for (int i = tid; i < a.D * (RT / 16); i += 256) {  // the capacity is a multiple of 16: whole pieces
+    const int d = i / (RT / 16), t = i % (RT / 16) * 4;
+    uint4 c = make_uint4(0, 0, 0, 0);
+    if (r0 + t * 4 < len) c = __ldg(reinterpret_cast<const uint4*>(v + (size_t)d * a.cap + r0 + t * 4));
+    uint32_t* row = words + d * (RT / 4);
+    const int mix = d / 8 % 16;
+    row[t ^ mix] = c.x, row[(t + 1) ^ mix] = c.y, row[(t + 2) ^ mix] = c.z, row[(t + 3) ^ mix] = c.w;
+  }
+  __syncthreads();
+  const int D8 = a.D / 8;
   for (int i = tid; i < D8 * (RT / 4); i += 256) {
-    const int r = r0 + i % (RT / 4) * 4, d = i / (RT / 4) * 8;
-    if (r >= a.rows) continue;
-    uint32_t w[8] = {};
-    float s = 0.f;
-    if (r < len) {  // the capacity is a multiple of 4, a block of 16: four tokens lie in both or in neither
-      s = __ldg(vs + r / a.block);
+    const int t4 = i / D8, d8 = i % D8, d = d8 * 8, r = r0 + t4 * 4;
+    const float s = r < len ? __ldg(vs + (r >> a.block_log2)) : 0.f;
+    uint32_t w[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = __ldg(reinterpret_cast<const uint32_t*>(v + (size_t)(d + j) * a.cap + r));
-    }
+    for (int j = 0; j < 8; ++j) w[j] = words[(d + j) * (RT / 4) + (t4 ^ (d8 % 16))];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       if (r + t >= a.rows) break;
@@ -363,12 +374,13 @@ extern "C" fa_status fa_kv8_read(const fa_kv8* c, const int* lens, int rows, voi
   if ((st = kv8_check_pointers(c)) != FA_OK) return st;
   if ((st = check_pointers({{"lens", lens}, {"k", k}, {"v", v}})) != FA_OK) return st;
   ReadArgs a{c->k, c->v, c->k_scale, c->v_scale, lens, k, v, rows, c->layers, c->heads, c->head_dim, c->capacity,
-             c->block};
+             c->block, __builtin_ctz(c->block)};
+  const size_t smem = (size_t)c->head_dim * RT;
   const dim3 grid((rows + RT - 1) / RT, c->heads, c->batch * c->layers);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == FA_DT_F32) read_kernel<float><<<grid, 256, 0, s>>>(a);
-  else if (dtype == FA_DT_BF16) read_kernel<bf16><<<grid, 256, 0, s>>>(a);
-  else read_kernel<__half><<<grid, 256, 0, s>>>(a);
+  if (dtype == FA_DT_F32) read_kernel<float><<<grid, 256, smem, s>>>(a);
+  else if (dtype == FA_DT_BF16) read_kernel<bf16><<<grid, 256, smem, s>>>(a);
+  else read_kernel<__half><<<grid, 256, smem, s>>>(a);
   FA_CUDA(nullptr, cudaGetLastError());
   return FA_OK;
 }

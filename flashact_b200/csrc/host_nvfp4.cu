@@ -11,7 +11,7 @@
 // A warp takes 16 * RT rows of W, and every eighth chunk of the CTA's whole K; the eight warps' sums meet in
 // shared memory in warp order. The order of k inside the matrix instruction is free as long as both
 // operands share it: a lane owns PB bytes of codes (one or two scale blocks) of each of its rows, read
-// with one load, and x's pairs (k, k + 4) follow the order in which the codes come out of a word.
+// with one load a turn ahead, and x's pairs follow the order in which the codes come out of a word.
 #include "fa_kv8.cuh"
 
 namespace {
@@ -27,22 +27,30 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The 16-bit type of x: where a code's bits go, and the powers of two that come with it.
+// bf16: a code's bits in place are its value times 2^-126, the scale goes in times 2^100, the rest at the end. fp16: values as they
+// are; code times scale lies between 2^-10 and 2688.
 template <bool HALF>
 struct Fmt {
-  // f16: code value * 2^-14, scale * 2^7 (448 * 2^7 is finite); bf16: * 2^-126, scale * 2^100
-  static constexpr int MAG = HALF ? 9 : 6;
-  static constexpr uint32_t MMASK = HALF ? 0x0E000E00u : 0x01C001C0u;
-  static constexpr float SCALE = HALF ? 128.0f : 1.2676506002282294e30f;
-  static constexpr float UNIT = HALF ? 128.0f : 67108864.0f;  // 2^7; 2^26
+  static constexpr float SCALE = HALF ? 1.0f : 1.2676506002282294e30f;  // 2^100
+  static constexpr float UNIT = HALF ? 1.0f : 67108864.0f;              // 2^26
 };
 
-// Codes i and i + 4 of a word, as the two halves.
+// Two codes of a word as the two halves: bf16 codes I and I + 4 (bits put in place), fp16 codes 2 I and 2 I + 1 (one conversion,
+// measured 2.2 cycles against 8 for the bits; there is none to bf16).
 template <bool HALF, int I>
 __device__ __forceinline__ uint32_t pair(uint32_t u) {
-  constexpr int M = Fmt<HALF>::MAG - 4 * I, S = 12 - 4 * I;
-  const uint32_t m = M >= 0 ? u << (M >= 0 ? M : 0) : u >> (M < 0 ? -M : 0);
-  return (m & Fmt<HALF>::MMASK) | ((u << S) & 0x80008000u);
+  if constexpr (HALF) {
+    uint32_t r;
+    if constexpr (I == 0) asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(r) : "r"(u));
+    if constexpr (I == 1) asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(r) : "r"(u));
+    if constexpr (I == 2) asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, c;\n\t}" : "=r"(r) : "r"(u));
+    if constexpr (I == 3) asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, d;\n\t}" : "=r"(r) : "r"(u));
+    return r;
+  } else {
+    constexpr int M = 6 - 4 * I, S = 12 - 4 * I;
+    const uint32_t m = M >= 0 ? u << (M >= 0 ? M : 0) : u >> (M < 0 ? -M : 0);
+    return (m & 0x01C001C0u) | ((u << S) & 0x80008000u);
+  }
 }
 template <bool HALF>
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
@@ -55,9 +63,7 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
 template <bool HALF, int N>
 __device__ __forceinline__ void factors(uint32_t two, uint32_t (&f)[N]) {
   uint32_t v = e4m3_lo_f16x2(two);
-  if constexpr (HALF) {
-    v = mul2<true>(v, 0x58005800u);  // 2^7
-  } else {
+  if constexpr (!HALF) {
     const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v));
     const __nv_bfloat162 y = __floats2bfloat162_rn(x.x * Fmt<false>::SCALE, x.y * Fmt<false>::SCALE);
     v = *reinterpret_cast<const uint32_t*>(&y);
@@ -82,7 +88,7 @@ struct LinArgs {
 };
 
 template <bool HALF, int PB, int MT, int RT>
-__global__ void __launch_bounds__(LW * 32) linear_kernel(const LinArgs a) {
+__global__ void __launch_bounds__(LW * 32, 2) linear_kernel(const LinArgs a) {
   constexpr int WORDS = PB / 4, PK = PB * 2, GROUPS = PK / 16;  // 32-bit words, k and scale blocks of a lane's piece
   __shared__ float part[LW][16 * RT][8 * MT + 1];
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -149,6 +155,10 @@ __global__ void __launch_bounds__(LW * 32) linear_kernel(const LinArgs a) {
       uint32_t b[MT][4];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
+        if constexpr (HALF) {
+          b[m][0] = xv[m][j].x, b[m][1] = xv[m][j].y, b[m][2] = xv[m][j].z, b[m][3] = xv[m][j].w;
+          continue;
+        }
         b[m][0] = __byte_perm(xv[m][j].x, xv[m][j].z, 0x5410);  // (x0, x4)
         b[m][1] = __byte_perm(xv[m][j].x, xv[m][j].z, 0x7632);  // (x1, x5)
         b[m][2] = __byte_perm(xv[m][j].y, xv[m][j].w, 0x5410);  // (x2, x6)
