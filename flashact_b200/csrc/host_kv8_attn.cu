@@ -102,12 +102,21 @@ fa_status attn_check(const fa_kv8* c, int tokens, int q_heads, int max_len) {
   return FA_OK;
 }
 
-int sm_count() {
-  int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+// SMs of the current device; 148 where there is none, so that a workspace can be sized anywhere.
+int sm_count(int* device = nullptr) {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
-    n = 148;
+    return 148;
   }
+  if (device) *device = dev;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 148;
+  }
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
@@ -138,7 +147,8 @@ extern "C" fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, in
     return fail(nullptr, FA_ERR_INVALID, "queries and output must be aligned to their type");
   if (tokens == 0) return FA_OK;
   const int top = max_len ? max_len : c->capacity;
-  const Plan p = make_plan(c, tokens, q_heads, top, sm_count());
+  int device = 0;
+  const Plan p = make_plan(c, tokens, q_heads, top, sm_count(&device));
   if (workspace_bytes < p.part_bytes + p.ml_bytes)
     return fail(nullptr, FA_ERR_INVALID, "workspace of %zu bytes, %zu are needed", workspace_bytes, p.part_bytes + p.ml_bytes);
   if (p.part_bytes && reinterpret_cast<uintptr_t>(workspace) % 16)
@@ -149,6 +159,7 @@ extern "C" fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, in
   if (prefix && (st = check_pointers({{"prefix", prefix}})) != FA_OK) return st;
   if (p.part_bytes && (st = check_pointers({{"workspace", workspace}})) != FA_OK) return st;
   AttnArgs a;
+  a.device = device;
   a.k = c->k, a.v = c->v, a.ks = c->k_scale, a.vs = c->v_scale;
   a.q = q->ptr, a.out = out->ptr;
   a.qb = q->batch, a.qt = q->token, a.qh = q->head;

@@ -18,6 +18,7 @@ struct AttnArgs {
   // Splits of the key axis, joined by the cluster that they are (at most 8), or by the merge kernel. With a cluster
   // each takes an equal share of the observation's own tiles, else tiles [split * split_chunks, + split_chunks).
   int nsplit, cluster, split_chunks;
+  int device;
   int rows;                  // rows of a tile
   int tiles;                 // row tiles of a (observation, key head)
   float* part;               // [slot][rows of a tile][D] unnormalised sums, slot = ((b, h), tile, split)

@@ -408,8 +408,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
 template <int R, bool HALF, int MT>
 fa_status launch(const AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
   constexpr int SMEM = Cfg<R, HALF, MT>::SMEM;
-  FA_CUDA(nullptr, cudaFuncSetAttribute(few_kernel<R, HALF, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-  return kv8_launch(few_kernel<R, HALF, MT>, a, batch, THREADS, SMEM, km, vm, s);
+  return kv8_launch<few_kernel<R, HALF, MT>>(a, batch, THREADS, SMEM, km, vm, s);
 }
 template <int R>
 fa_status launch_rows(const AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {

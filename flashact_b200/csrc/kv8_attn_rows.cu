@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 template <bool HALF, int MT>
 fa_status launch(const AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
   constexpr int SMEM = Cfg<HALF, MT>::SMEM;
-  return kv8_launch(rows_kernel<HALF, MT>, a, batch, THREADS, SMEM, km, vm, s);
+  return kv8_launch<rows_kernel<HALF, MT>>(a, batch, THREADS, SMEM, km, vm, s);
 }
 
 }  // namespace

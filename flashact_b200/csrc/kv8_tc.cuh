@@ -1,6 +1,8 @@
 // What the two tensor-core attention kernels over the 8-bit cache share: tile loads, the 8-bit matrix instruction, the
 // splitting of queries and probabilities into 8-bit parts.
 #pragma once
+#include <atomic>
+
 #include "kv8_attn.cuh"
 
 namespace fa {
@@ -285,10 +287,9 @@ __device__ __forceinline__ void produce(unsigned char* ring, uint64_t* full, uin
 }  // namespace kv8
 }  // namespace fa
 
-template <class Kernel>
-static fa_status kv8_launch(Kernel kernel, const fa::kv8::AttnArgs& a, int batch, int threads, int smem, const CUtensorMap& km,
+template <auto kernel>
+static fa_status kv8_launch(const fa::kv8::AttnArgs& a, int batch, int threads, int smem, const CUtensorMap& km,
                             const CUtensorMap& vm, cudaStream_t s) {
-  FA_CUDA(nullptr, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.nsplit * a.tiles, a.heads, batch);
   cfg.blockDim = dim3(threads);
@@ -300,6 +301,13 @@ static fa_status kv8_launch(Kernel kernel, const fa::kv8::AttnArgs& a, int batch
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = a.cluster ? 1 : 0;
+  // The shared memory limit is set on a device's first launch of a kernel, and again where a launch fails (a device that was reset).
+  static std::atomic<unsigned long long> set{0};
+  const unsigned long long bit = 1ull << (a.device & 63);
+  if ((set.load(std::memory_order_relaxed) & bit) && cudaLaunchKernelEx(&cfg, kernel, a, km, vm) == cudaSuccess) return FA_OK;
+  cudaGetLastError();
+  FA_CUDA(nullptr, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   FA_CUDA(nullptr, cudaLaunchKernelEx(&cfg, kernel, a, km, vm));
+  set.fetch_or(bit, std::memory_order_relaxed);
   return FA_OK;
 }

@@ -12,12 +12,11 @@ from . import _capi as C
 from .pi05 import _DT
 
 _byref = ctypes.byref
-_current_device = torch.cuda.current_device
+_current_device = torch._C._cuda_getDevice
 
 
-def _current_stream(index):
-    """The raw current stream of a device: what torch.cuda.current_stream(index).cuda_stream gives, without the object."""
-    return torch._C._cuda_getCurrentRawStream(index)
+# the raw current stream of a device: torch.cuda.current_stream(index).cuda_stream without the object
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _bad(msg):
@@ -97,7 +96,7 @@ class Kv8Cache:
         shape = t.shape
         if len(shape) != 4 or shape[0] != self.batch or shape[2] != heads or shape[3] != self.head_dim:
             raise _bad(f"'{name}' must be [{self.batch}][tokens][{heads}][{self.head_dim}], got {tuple(shape)}")
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise _bad(f"'{name}' is on {t.device}, the cache on {self.device}")
         st = t.stride()
         if st[3] != 1:
@@ -108,7 +107,7 @@ class Kv8Cache:
     def _ints(self, name, t):
         if t is None:
             return None
-        if t.dtype != torch.int32 or t.shape != self._lens_tensor.shape or not t.is_contiguous() or t.device != self.device:
+        if t.dtype != torch.int32 or t.shape != self._lens_tensor.shape or not t.is_contiguous() or t.get_device() != self._index:
             raise _bad(f"'{name}' must be a contiguous int32 tensor [{self.batch}] on {self.device}")
         return t.data_ptr()
 
@@ -152,8 +151,8 @@ class Kv8Cache:
             raise _bad(f"q must be a bf16 or fp16 tensor of four dimensions, got {q.dtype} {tuple(shape)}")
         tokens, q_heads = shape[1], shape[2]
         q, qr = self._rows("q", q, q_heads)
-        if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=self.device)
+        if out is None:  # contiguous like q, or of its own where q is not
+            out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
             if q_lens is not None:
                 out.zero_()
         elif out.shape != shape or out.dtype != q.dtype or out.device != self.device or (out.numel() and out.stride(3) != 1):
@@ -182,7 +181,8 @@ class Kv8Cache:
         if rows < 0:
             raise _bad(f"rows={rows}")
         shape = (self.batch, self.layers, rows, self.heads * self.head_dim)
-        k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
+        k = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
         self._check(self.lib.fa_kv8_read(self._ref, self._lens if lens is None else self._ints("lens", lens), rows, k.data_ptr(),
                                          v.data_ptr(), _DT[dtype], _current_stream(self._index)))
         return k, v

@@ -63,36 +63,43 @@ def nvfp4_linear(x: torch.Tensor, packed: torch.Tensor, block_scale: torch.Tenso
     """x W^T * tensor_scale (+ bias) for x [..., K] (bf16 or fp16) of up to 16 rows and one layer's matrix as
     quantize_nvfp4 gives it: packed uint8 [N, K/2], block_scale uint8 [N, K/16], tensor_scale fp32 of one element;
     bias fp32 [N]. Returns [..., N] in x's type."""
-    dt, shape, dev = _DT.get(x.dtype), x.shape, x.device
-    if dt is None or not shape or not x.is_cuda:
+    dt, shape, index = _DT.get(x.dtype), x.shape, x.get_device()
+    if dt is None or not shape or index < 0:
         raise C.FlashActError(C.FA_ERR_INVALID, "x must be a CUDA tensor [..., K]")
-    if stream is not None or torch.cuda.current_device() != dev.index:
-        with torch.cuda.stream(stream) if stream is not None else torch.cuda.device(dev):
+    if stream is not None or torch._C._cuda_getDevice() != index:
+        with torch.cuda.stream(stream) if stream is not None else torch.cuda.device(index):
             return nvfp4_linear(x, packed, block_scale, tensor_scale, bias=bias, out=out)
     K, pshape = shape[-1], packed.shape
     N = pshape[0] if len(pshape) == 2 else 0
-    _operand("packed", packed, (N, K // 2), torch.uint8, dev)
-    _operand("block_scale", block_scale, (N, K // 16), torch.uint8, dev)
-    _operand("tensor_scale", tensor_scale, None, torch.float32, dev)
-    if bias is not None:
-        _operand("bias", bias, (N,), torch.float32, dev)
-    shape = (*shape[:-1], N)
+    if (pshape != (N, K // 2) or packed.dtype != torch.uint8 or packed.get_device() != index or not packed.is_contiguous()
+            or block_scale.shape != (N, K // 16) or block_scale.dtype != torch.uint8 or block_scale.get_device() != index
+            or not block_scale.is_contiguous() or tensor_scale.numel() != 1 or tensor_scale.dtype != torch.float32
+            or tensor_scale.get_device() != index or bias is not None
+            and (bias.shape != (N,) or bias.dtype != torch.float32 or bias.get_device() != index or not bias.is_contiguous())):
+        _bad_operand(x, ("packed", packed, (N, K // 2), torch.uint8), ("block_scale", block_scale, (N, K // 16), torch.uint8),
+                     ("tensor_scale", tensor_scale, None, torch.float32), ("bias", bias, (N,), torch.float32))
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=dev)
-    elif out.shape != shape or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
-        raise C.FlashActError(C.FA_ERR_INVALID, f"'out' must be a contiguous {x.dtype} tensor {tuple(shape)} on {dev}")
+        out = x.new_empty((*shape[:-1], N))
+    elif out.shape != (*shape[:-1], N) or out.dtype != x.dtype or out.get_device() != index or not out.is_contiguous():
+        raise C.FlashActError(C.FA_ERR_INVALID, f"'out' must be a contiguous {x.dtype} tensor {(*shape[:-1], N)} on {x.device}")
     if not x.is_contiguous():
         x = x.contiguous()
-    if x.data_ptr() % 16:
+    p = x.data_ptr()
+    if p % 16:
         x = x.clone()
+        p = x.data_ptr()
     lib = C.load_library()
-    _check(lib, lib.fa_nvfp4_linear(x.data_ptr(), dt, x.numel() // K if K else 0, K, K, packed.data_ptr(), block_scale.data_ptr(),
-                                    tensor_scale.data_ptr(), None if bias is None else bias.data_ptr(), N, out.data_ptr(), N,
-                                    torch._C._cuda_getCurrentRawStream(dev.index)))
+    st = lib.fa_nvfp4_linear(p, dt, x.numel() // K if K else 0, K, K, packed.data_ptr(), block_scale.data_ptr(), tensor_scale.data_ptr(),
+                             None if bias is None else bias.data_ptr(), N, out.data_ptr(), N,
+                             torch._C._cuda_getCurrentRawStream(index))
+    if st != C.FA_OK:
+        _check(lib, st)
     return out
 
 
-def _operand(name, t, shape, dtype, dev):
-    if (t.numel() != 1 if shape is None else t.shape != shape) or t.dtype != dtype or t.device != dev or not t.is_contiguous():
-        raise C.FlashActError(C.FA_ERR_INVALID, f"'{name}' must be a contiguous {dtype} tensor {shape or '(one element)'} on {dev}, "
-                                                f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _bad_operand(x, *operands):
+    for name, t, shape, dtype in operands:
+        if t is not None and ((t.numel() != 1 if shape is None else t.shape != shape) or t.dtype != dtype or t.device != x.device
+                              or not t.is_contiguous()):
+            raise C.FlashActError(C.FA_ERR_INVALID, f"'{name}' must be a contiguous {dtype} tensor {shape or '(one element)'} on "
+                                                    f"{x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
