@@ -228,7 +228,7 @@ extern "C" fa_status fa_nvfp4_linear(const void* x, fa_dtype dtype, int M, int K
                                      void* y, long long ldy, fa_stream stream) {
   if (dtype != FA_DT_BF16 && dtype != FA_DT_F16)
     return fail(nullptr, FA_ERR_UNSUPPORTED, "x is bf16 or fp16 (dtype %d)", (int)dtype);
-  if (M < 0 || N < 1 || K < 1) return fail(nullptr, FA_ERR_INVALID, "shape M=%d N=%d K=%d", M, N, K);
+  if (M < 0 || N < 1 || K < 1 || N > (1 << 30) || K > (1 << 30)) return fail(nullptr, FA_ERR_INVALID, "shape M=%d N=%d K=%d", M, N, K);
   if (M > 16) return fail(nullptr, FA_ERR_UNSUPPORTED, "M=%d rows: up to 16 are a matrix-vector product", M);
   if (K % 16) return fail(nullptr, FA_ERR_INVALID, "K=%d is not a multiple of 16", K);
   if ((M > 1 && ldx < K) || ldx % 8) return fail(nullptr, FA_ERR_INVALID, "ldx=%lld for K=%d (a multiple of 8)", ldx, K);

@@ -304,8 +304,10 @@ static fa_status kv8_launch(const fa::kv8::AttnArgs& a, int batch, int threads, 
   // The shared memory limit is set on a device's first launch of a kernel, and again where a launch fails (a device that was reset).
   static std::atomic<unsigned long long> set{0};
   const unsigned long long bit = 1ull << (a.device & 63);
-  if ((set.load(std::memory_order_relaxed) & bit) && cudaLaunchKernelEx(&cfg, kernel, a, km, vm) == cudaSuccess) return FA_OK;
-  cudaGetLastError();
+  if (set.load(std::memory_order_relaxed) & bit) {
+    if (cudaLaunchKernelEx(&cfg, kernel, a, km, vm) == cudaSuccess) return FA_OK;
+    cudaGetLastError();
+  }
   FA_CUDA(nullptr, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   FA_CUDA(nullptr, cudaLaunchKernelEx(&cfg, kernel, a, km, vm));
   set.fetch_or(bit, std::memory_order_relaxed);

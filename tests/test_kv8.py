@@ -247,6 +247,51 @@ def test_attention_masks(require_gpu, dtype):
     _check(cache.attend(0, q.cuda(), causal=False, lens=dev([3] * B)), want, tol)
 
 
+def _workspace(tokens, q_heads, cap, max_len=0, **kw):
+    from flashact_b200 import _capi as C
+    from flashact_b200.build import build
+    n = ctypes.c_size_t()
+    c = _desc(capacity=cap, **kw)
+    assert C.load_library(build()).fa_kv8_attention_workspace(ctypes.byref(c), tokens, q_heads, max_len, ctypes.byref(n)) == 0
+    return n.value
+
+
+def test_workspace_follows_the_splits():
+    """More than eight splits of the keys go through the merge kernel and a workspace; up to eight are a cluster."""
+    one = dict(batch=1, layers=1, heads=1, head_dim=64)
+    assert _workspace(1, 4, 1 << 16, **one) > 0 and _workspace(40, 4, 1 << 16, **one) > 0
+    assert _workspace(1, 4, 1 << 16, max_len=1024, **one) == 0
+    assert _workspace(1, 64, 1 << 15, batch=64, layers=1, heads=8, head_dim=128) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("T,H,D", [(1, 4, 64), (3, 4, 96), (40, 4, 64), (33, 4, 256)])
+def test_attention_many_splits(require_gpu, T, H, D, dtype):
+    """A long cache of one key head: splits joined by the merge kernel, some of them without a key; the captured call follows
+    the lengths into other numbers of splits."""
+    cap, lens, q_lens = 1 << 15, [20000, 130, 0], [T, T, max(1, T - 2)]
+    assert _workspace(T, H, cap, batch=3, layers=1, heads=1, head_dim=D) > 0
+    ref = random_ref(3, 1, 1, D, cap, 128, D)
+    cache, q = ref.to_cache(lens), _q((3, T, H, D), dtype, 3)
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    ql, prefix, qc = dev(q_lens), dev([40, 0, 7]), q.cuda()
+    out = torch.zeros(3, T, H, D, dtype=dtype, device="cuda")
+    cache.attend(0, qc, q_lens=ql, prefix=prefix, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        cache.attend(0, qc, q_lens=ql, prefix=prefix, out=out)
+    for now in (lens, [700, 20, 5000]):
+        cache.lens.copy_(dev(now))
+        out.fill_(5.0)
+        g.replay()
+        want, tol = attend(ref, 0, q, now, prefix=[40, 0, 7], q_lens=q_lens)
+        for b in range(3):
+            _check(out[b, :q_lens[b]], want[b, :q_lens[b]], tol[b, :q_lens[b]])
+            assert (out[b, q_lens[b]:] == 5.0).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,H,D", [(1, 8, 256), (40, 8, 64)])
 def test_attention_layouts(require_gpu, T, H, D):
