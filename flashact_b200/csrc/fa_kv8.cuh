@@ -18,17 +18,6 @@ __device__ __forceinline__ uint32_t e4m3_lo_f16x2(uint32_t four) {
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(four));
   return r;
 }
-__device__ __forceinline__ uint32_t e4m3_hi_f16x2(uint32_t four) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(four));
-  return r;
-}
-// An 8x8 matrix of 16-bit values, two neighbours of row (lane / 4) in a lane's word, turned around.
-__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
-  uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
 
 // D(16x8, f32) += A(16x16, f16) B(16x8, f16).
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -59,14 +48,6 @@ __device__ __forceinline__ float log2_approx(float x) {
 __device__ __forceinline__ void cp_async16_zfill(void* smem_dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem_dst)), "l"(src), "r"(on ? 16 : 0)
                : "memory");
-}
-__device__ __forceinline__ void cp_async8_zfill(void* smem_dst, const void* src, bool on) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(smem_dst)), "l"(src), "r"(on ? 8 : 0)
-               : "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait_group() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // Keys of a query: j < limit, limit = min(len, max(position + 1, prefix)); full masks see all len keys.

@@ -168,6 +168,7 @@ extern "C" fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, in
   a.layers = c->layers, a.layer = layer, a.heads = c->heads, a.group = q_heads / c->heads, a.dim = c->head_dim, a.cap = c->capacity;
   a.blocks = c->capacity / c->block, a.block_log2 = __builtin_ctz(c->block), a.half = dtype == FA_DT_F16;
   a.q_wide = reinterpret_cast<uintptr_t>(q->ptr) % 16 == 0 && q->batch % 8 == 0 && q->token % 8 == 0 && q->head % 8 == 0;
+  a.o_wide = reinterpret_cast<uintptr_t>(out->ptr) % 8 == 0 && out->batch % 4 == 0 && out->token % 4 == 0 && out->head % 4 == 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.group_mul = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
   a.nsplit = p.nsplit, a.cluster = p.cluster, a.split_chunks = p.split_chunks, a.rows = p.rows, a.tiles = p.tiles;

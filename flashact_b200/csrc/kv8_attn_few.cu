@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
     if (a.nsplit > 1 && !a.cluster && split > 0) return;  // the merge knows
     for (int i = tid; i < R * PITCH; i += THREADS) osum[i] = 0.f;
     if (tid < R) mls[tid] = make_float2(-INFINITY, 0.f);
-    finish_rows<HALF, MT>(a, osum, PITCH, reinterpret_cast<const float*>(mls), 2, split, b, h, row0, nrows, n, nq, pre, first_part);
+    finish_rows<HALF, MT, 1>(a, osum, PITCH, reinterpret_cast<const float*>(mls), 2, split, b, h, row0, nrows, n, nq, pre, first_part);
     return;
   }
 
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
   }
   __syncthreads();
   if (w == 1) tmem_dealloc(tmem, C::COLS);
-  finish_rows<HALF, MT>(a, osum, PITCH, reinterpret_cast<const float*>(mls), 2, split, b, h, row0, nrows, n, nq, pre, first_part);
+  finish_rows<HALF, MT, 1>(a, osum, PITCH, reinterpret_cast<const float*>(mls), 2, split, b, h, row0, nrows, n, nq, pre, first_part);
 }
 
 template <int R, bool HALF, int MT>

@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (nt <= 0) {  // nothing left for this split
     if (a.nsplit > 1 && !a.cluster && split > 0) return;  // the merge knows
     for (int i = tid; i < ROWS * PITCH; i += THREADS) osum[i] = i % PITCH == MT * 128 ? -INFINITY : 0.f;
-    finish_rows<HALF, MT>(a, osum, PITCH, osum + MT * 128, PITCH, split, b, h, row0, nrows, n, nq, pre, first_part);
+    finish_rows<HALF, MT, 4>(a, osum, PITCH, osum + MT * 128, PITCH, split, b, h, row0, nrows, n, nq, pre, first_part);
     return;
   }
 
@@ -108,51 +108,97 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   float vref = 0.f;  // largest V scale of the split
   if (w >= SOFT) {
-    const int kend = min(top, (t0 + nt) * TILE);
-    for (int i = ((t0 * TILE) >> a.block_log2) + tid - SOFT * 32; (i << a.block_log2) < kend; i += 256) vref = fmaxf(vref, vs[i]);
     // queries: power-of-two row scales and E4M3 parts; rows behind the last are zero
     constexpr int LANES = MT * 16, PER = 32 / LANES, N = 16 / PER;  // lanes of a row, rows at a time, such groups of the warp's 16 rows
     const int l8 = (lane % LANES) * 8;                              // this lane's dims, l8 .. + 7
-    auto source = [&](int j) {
-      const int r = row0 + (w - SOFT) * 16 + j * PER + lane / LANES;
-      return token_of(a, r) < a.mask.tokens && l8 < a.dim
-                 ? reinterpret_cast<const uint16_t*>(a.q) + row_at(a, b, h, r, a.qb, a.qt, a.qh) + l8 : nullptr;
+    // row addresses by the first 16 lanes, once; zero for rows that the call does not have
+    unsigned long long at = 0;
+    {
+      const int r = row0 + (w - SOFT) * 16 + (lane & 15);
+      if (token_of(a, r) < a.mask.tokens)
+        at = reinterpret_cast<unsigned long long>(reinterpret_cast<const uint16_t*>(a.q) + row_at(a, b, h, r, a.qb, a.qt, a.qh));
+    }
+    // A row as it is waits where its parts will be (512 bytes either way at head_dim 256): all rows are on their way at once.
+    auto place = [&](int j) {
+      const int r = (w - SOFT) * 16 + j * PER + lane / LANES, piece = lane % LANES;
+      return reinterpret_cast<uint4*>(qs + (piece >> 3) * 16384 + swz(r, (piece & 7) * 16));
     };
-    auto split = [&](int j, uint4 q) {
-      const int r = (w - SOFT) * 16 + j * PER + lane / LANES;
-      const float2 x0 = pair_f32<HALF>(q.x), x1 = pair_f32<HALF>(q.y), x2 = pair_f32<HALF>(q.z), x3 = pair_f32<HALF>(q.w);
-      float m = fmaxf(fmaxf(fmaxf(fabsf(x0.x), fabsf(x0.y)), fmaxf(fabsf(x1.x), fabsf(x1.y))),
-                      fmaxf(fmaxf(fabsf(x2.x), fabsf(x2.y)), fmaxf(fabsf(x3.x), fabsf(x3.y))));
+    if (a.q_wide) {
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      for (int j = 0; j < N; ++j) {
+        const unsigned long long base = __shfl_sync(0xffffffffu, at, j * PER + lane / LANES);
+        const bool on = base && l8 < a.dim;
+        cp_async16_zfill(place(j), on ? reinterpret_cast<const void*>(base + l8 * 2) : a.q, on);
+      }
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < N; ++j) {
+        const unsigned long long base = __shfl_sync(0xffffffffu, at, j * PER + lane / LANES);
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + l8;
+        uint32_t u[4] = {0, 0, 0, 0};
+        if (base && l8 < a.dim) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) u[k] = (uint32_t)__ldg(p + 2 * k) | ((uint32_t)__ldg(p + 2 * k + 1) << 16);
+        }
+        *place(j) = make_uint4(u[0], u[1], u[2], u[3]);
+        __syncwarp();
+      }
+    }
+    auto largest = [&](uint4 q) {
+      const float2 x[4] = {pair_f32<HALF>(q.x), pair_f32<HALF>(q.y), pair_f32<HALF>(q.z), pair_f32<HALF>(q.w)};
+      return max3(max3(fabsf(x[0].x), fabsf(x[0].y), fabsf(x[1].x)), max3(fabsf(x[1].y), fabsf(x[2].x), fabsf(x[2].y)),
+                  fmaxf(fabsf(x[3].x), fabsf(x[3].y)));
+    };
+    auto split = [&](int j, uint4 q, float m) {
+      const int r = (w - SOFT) * 16 + j * PER + lane / LANES;
+      const float2 x[4] = {pair_f32<HALF>(q.x), pair_f32<HALF>(q.y), pair_f32<HALF>(q.z), pair_f32<HALF>(q.w)};
       float back;
       const float up = row_factor(m, back), mul = r < nrows ? copysignf(up, a.scale_log2) : 0.f;
       if (l8 == 0) rowscale[r] = back * fabsf(a.scale_log2);
-      float y[4] = {x0.x * mul, x0.y * mul, x1.x * mul, x1.y * mul}, z[4] = {x2.x * mul, x2.y * mul, x3.x * mul, x3.y * mul};
-      uint32_t e[C::QP];
-      split_query<C::QP>(y, 1.f, [&](int p, uint32_t v) { e[p] = v; });
-      split_query<C::QP>(z, 1.f, [&](int p, uint32_t v) {
-        *reinterpret_cast<uint2*>(qs + (p * MT + (l8 >> 7)) * 16384 + swz(r, l8 & 127)) = make_uint2(e[p], v);
-      });
-    };
-    auto load = [&](int j) {
-      const uint16_t* p = j < N ? source(j) : nullptr;
-      if (!p) return make_uint4(0, 0, 0, 0);
-      if (a.q_wide) return __ldg(reinterpret_cast<const uint4*>(p));
-      uint32_t u[4];
+      // scaled elements are f16 numbers (what is below 2^-24 is far below the parts' end), and so are the remainders
+      uint32_t y[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) u[k] = (uint32_t)__ldg(p + 2 * k) | ((uint32_t)__ldg(p + 2 * k + 1) << 16);
-      return make_uint4(u[0], u[1], u[2], u[3]);
+      for (int k = 0; k < 4; ++k) y[k] = pack_f16x2(x[k].x * mul, x[k].y * mul);
+      unsigned char* dst = qs + (l8 >> 7) * 16384 + swz(r, l8 & 127);
+#pragma unroll
+      for (int p = 0; p < C::QP; ++p) {
+        uint32_t e[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          e[k] = f16x2_e4m3x2(y[k]);
+          if (p + 1 < C::QP) {
+            const uint32_t v = e4m3_lo_f16x2(e[k]);
+            const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&y[k]), *reinterpret_cast<const __half2*>(&v));
+            y[k] = *reinterpret_cast<const uint32_t*>(&d);
+          }
+        }
+        *reinterpret_cast<uint2*>(dst + p * MT * 16384) = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
+      }
     };
-    // two rows (or pairs of rows) a turn, the next two on their way; rolled, since straight code would be fetched cold
-    uint4 q0 = load(0), q1 = load(1);
+    const int kend = min(top, (t0 + nt) * TILE);
+    for (int i = ((t0 * TILE) >> a.block_log2) + tid - SOFT * 32; (i << a.block_log2) < kend; i += 256) vref = fmaxf(vref, vs[i]);
+    cp_async_wait_all();
+    __syncwarp();
 #pragma unroll 1
-    for (int j = 0; j < N; j += 2) {
-      const uint4 n0 = load(j + 2), n1 = load(j + 3);
+    for (int j0 = 0; j0 < N; j0 += 4) {  // four rows' chains side by side; all in straight code would be fetched cold
+      uint4 q[4];
+      float m[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[j] = *place(j0 + j);
       __syncwarp();
-      split(j, q0);
-      split(j + 1, q1);
-      q0 = n0, q1 = n1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m[j] = largest(q[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (MT == 2) {
+          m[j] = warp_max(m[j]);
+        } else {
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) m[j] = fmaxf(m[j], __shfl_xor_sync(0xffffffffu, m[j], o));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) split(j0 + j, q[j], m[j]);
     }
     fence_proxy_async_shared();
     vref = warp_max(vref);
@@ -215,15 +261,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     const float rs = rowscale[row];
     const int lim = row < nrows ? a.mask.limit(n, nq, pre, token_of(a, row0 + row)) : 0;
 
-    float kn[4], vn[4];  // scales of the four 16-key groups of this half, a tile ahead
+    float next = 0.f;  // lanes 0..3: K scales of this half's four 16-key groups in the next tile, lanes 4..7: V scales
     auto scales = [&](int i) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = (t0 + i) * TILE + half * 64 + 16 * j;
-        const bool live = i < nt && key < top;
-        kn[j] = live ? __ldg(ks + (key >> a.block_log2)) : 0.f;
-        vn[j] = live ? __ldg(vs + (key >> a.block_log2)) : 0.f;
-      }
+      const int key = (t0 + i) * TILE + half * 64 + 16 * (lane & 3);
+      next = lane < 8 && i < nt && key < top ? __ldg((lane < 4 ? ks : vs) + (key >> a.block_log2)) : 0.f;
     };
     scales(0);
     float m = -INFINITY, l = 0.f;  // the subtracted maximum (the same in a row's two threads), this half's sum
@@ -244,8 +285,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (lane == 0) mbar_arrive(sfree);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        f[j] = rs * kn[j];
-        vf[j] = vn[j] * vinv;
+        f[j] = rs * __shfl_sync(0xffffffffu, next, j);
+        vf[j] = __shfl_sync(0xffffffffu, next, 4 + j) * vinv;
       }
       if ((t0 + i) * TILE + TILE > low) {  // not seen by every row
         const int left = lim - (t0 + i) * TILE - half * 64;
@@ -303,14 +344,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         // p vs / vref 2^14 straight from the exponent; the sum of p is that of a group over its factor. A factor below 2^-40 counts as
         // that: such a P is 0 in f16 either way.
         const float v = vf[j] < 9.094947e-13f ? 9.094947e-13f : vf[j], lv = log2_approx(v);
-        const uint64_t ff = pack2(f[j], f[j]), cc = pack2(lv - base, lv - base);
-        uint64_t g = 0;
+        const float cc = lv - base;
+        float g0 = 0.f, g1 = 0.f;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const float* x = s + 16 * j + 4 * c;
-          const float2 y = unpack2(fma2(pack2(x[0], x[1]), ff, cc)), z = unpack2(fma2(pack2(x[2], x[3]), ff, cc));
-          const float x0 = exp2_approx(y.x), x1 = exp2_approx(y.y), x2 = exp2_approx(z.x), x3 = exp2_approx(z.y);
-          g = add2(g, add2(pack2(x0, x1), pack2(x2, x3)));
+          const float x0 = exp2_approx(fmaf(x[0], f[j], cc)), x1 = exp2_approx(fmaf(x[1], f[j], cc));
+          const float x2 = exp2_approx(fmaf(x[2], f[j], cc)), x3 = exp2_approx(fmaf(x[3], f[j], cc));
+          g0 += x0 + x1;
+          g1 += x2 + x3;
           uint32_t p = pack_f16x2(x0, x1), q = pack_f16x2(x2, x3);
 #pragma unroll
           for (int k = 0; k < C::PP; ++k) {
@@ -319,8 +361,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (k + 1 < C::PP) p = rest1(p), q = rest1(q);
           }
         }
-        const float2 sum = unpack2(g);
-        l += (sum.x + sum.y) * exp2_approx(-lv);
+        l += (g0 + g1) * exp2_approx(-lv);
       }
       if (i + 1 < nt) fetch(i + 1);
       if (!ok) break;
@@ -369,7 +410,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   __syncthreads();
   if (w == 1) tmem_dealloc(tmem_o, 512);
-  finish_rows<HALF, MT>(a, osum, PITCH, osum + MT * 128, PITCH, split, b, h, row0, nrows, n, nq, pre, first_part);
+  finish_rows<HALF, MT, 4>(a, osum, PITCH, osum + MT * 128, PITCH, split, b, h, row0, nrows, n, nq, pre, first_part);
 }
 
 template <bool HALF, int MT>

@@ -53,27 +53,6 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
 }
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ uint64_t pack2(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-  return r;
-}
 __device__ __forceinline__ float warp_max(float x) {
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
@@ -97,6 +76,11 @@ __device__ __forceinline__ uint32_t rest8(uint32_t p) {  // eight times that: at
   const uint32_t d = rest1(p);
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&d), __float2half2_rn(8.f));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t f16x2_e4m3x2(uint32_t v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(v));
+  return r;
 }
 // A query's four scaled elements in E4M3 parts, each what the ones before left over, times `up`.
 template <int PARTS, class Store>
@@ -151,17 +135,17 @@ __device__ __forceinline__ float4 peer_f32x4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
-// Four consecutive 16-bit outputs of a row that may be 2-byte aligned only.
+// Four consecutive 16-bit outputs of a row; `wide`: 8-byte aligned.
 template <bool HALF>
-__device__ __forceinline__ void store16x4(uint16_t* p, float x, float y, float z, float w) {
+__device__ __forceinline__ void store16x4(uint16_t* p, const float (&v)[4], bool wide) {
   uint2 u;
   if constexpr (HALF) {
-    u = make_uint2(pack_f16x2(x, y), pack_f16x2(z, w));
+    u = make_uint2(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]));
   } else {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(x, y), b = __floats2bfloat162_rn(z, w);
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
     u = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
   }
-  if ((reinterpret_cast<uintptr_t>(p) & 7) == 0) {
+  if (wide) {
     *reinterpret_cast<uint2*>(p) = u;
   } else {
     p[0] = (uint16_t)u.x, p[1] = (uint16_t)(u.x >> 16);
@@ -170,8 +154,10 @@ __device__ __forceinline__ void store16x4(uint16_t* p, float x, float y, float z
 }
 // The end of a tile of rows: sums `o` [rows][pitch] relative to their maxima, and (maximum, sum) `ml`, in shared memory.
 // More than eight splits leave both for the merge kernel. Otherwise the splits, a cluster (or the only CTA), are joined in
-// split order, its CTAs sharing the output; a warp takes 128 dims of a row. All threads of all the CTAs come here.
-template <bool HALF, int MT>
+// split order, its CTAs sharing the output; a warp takes 128 dims of GROUP rows at a time. All threads of all the CTAs come here.
+// With up to 16 rows each row has a warp of its own, and what counts is the chain (0.3 us less than the other form takes for one
+// row of 8 us); with 128, four rows at a time keep enough loads on their way (13 us of a lone CTA's 36 with one, 5 with four).
+template <bool HALF, int MT, int GROUP>
 __device__ __forceinline__ void finish_rows(const AttnArgs& a, const float* o, int pitch, const float* ml, int ml_pitch, int rank,
                                             int b, int h, int row0, int nrows, int n, int nq, int pre, size_t first_part) {
   if (a.nsplit > 1 && !a.cluster) {
@@ -185,30 +171,76 @@ __device__ __forceinline__ void finish_rows(const AttnArgs& a, const float* o, i
     return;
   }
   cluster_sync();
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  for (int u = rank * warps + (threadIdx.x >> 5); u < nrows * MT; u += a.nsplit * warps) {
-    const int r = u / MT, d = (u % MT) * 128 + lane * 4, row = row0 + r;
-    // lane k weighs split k: none of it where the split has left no key to the row; a NaN in its sum stays
-    float2 x = make_float2(-INFINITY, 0.f);
-    if (lane < a.nsplit) x = peer_f32x2(peer(ml + r * ml_pitch, lane));
-    const bool none = x.x == -INFINITY && x.y == 0.f;
-    const float top = warp_max(x.x), f = none ? 0.f : exp2_approx(x.x - (top == -INFINITY ? 0.f : top));
-    const uint32_t live = __ballot_sync(0xffffffffu, !none);
-    float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, k8 = lane & 7;
+  const int groups = (nrows + GROUP - 1) / GROUP;
+  for (int u = rank * warps + (threadIdx.x >> 5); u < groups * MT; u += a.nsplit * warps) {
+    const int r0 = u / MT * GROUP, d = (u % MT) * 128 + lane * 4;
+    if constexpr (GROUP == 1) {  // lane k weighs split k
+      float2 x = make_float2(-INFINITY, 0.f);
+      if (lane < a.nsplit) x = peer_f32x2(peer(ml + r0 * ml_pitch, lane));
+      const bool none = x.x == -INFINITY && x.y == 0.f;
+      const float top = warp_max(x.x), f = none ? 0.f : exp2_approx(x.x - (top == -INFINITY ? 0.f : top));
+      const uint32_t live = __ballot_sync(0xffffffffu, !none);
+      float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float fk = __shfl_sync(0xffffffffu, f, k), lk = __shfl_sync(0xffffffffu, x.y, k);
-      if (live >> k & 1) {
-        sum += fk * lk;
-        const float4 p = peer_f32x4(peer(o + r * pitch + d, k));
-        v[0] += fk * p.x, v[1] += fk * p.y, v[2] += fk * p.z, v[3] += fk * p.w;
+      for (int k = 0; k < 8; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, k), lk = __shfl_sync(0xffffffffu, x.y, k);
+        if (live >> k & 1) {
+          sum += fk * lk;
+          const float4 p = peer_f32x4(peer(o + r0 * pitch + d, k));
+          v[0] += fk * p.x, v[1] += fk * p.y, v[2] += fk * p.z, v[3] += fk * p.w;
+        }
       }
+      const float norm = a.mask.limit(n, nq, pre, token_of(a, row0 + r0)) > 0 ? 1.0f / sum : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = norm == 0.f && sum == sum ? 0.f : v[i] * norm;
+      if (d < a.dim)
+        store16x4<HALF>(reinterpret_cast<uint16_t*>(a.out) + row_at(a, b, h, row0 + r0, a.ob, a.ot, a.oh) + d, v, a.o_wide);
+      continue;
     }
-    const float norm = a.mask.limit(n, nq, pre, token_of(a, row)) > 0 ? 1.0f / sum : 0.f;
-    if (norm == 0.f && sum == sum) v[0] = v[1] = v[2] = v[3] = 0.f;
-    if (d < a.dim)
-      store16x4<HALF>(reinterpret_cast<uint16_t*>(a.out) + row_at(a, b, h, row, a.ob, a.ot, a.oh) + d, v[0] * norm, v[1] * norm,
-                      v[2] * norm, v[3] * norm);
+    // lane 8 j + k weighs split k in row r0 + j: none of it where the split has left no key to the row; a NaN in its sum stays
+    const int r = min(r0 + (lane >> 3), nrows - 1), row = row0 + r;
+    float2 x = make_float2(-INFINITY, 0.f);
+    if (k8 < a.nsplit) x = peer_f32x2(peer(ml + r * ml_pitch, k8));
+    constexpr int STEP = 8 / GROUP;
+    float4 p[STEP][GROUP];
+    auto fetch = [&](int k0) {
+#pragma unroll
+      for (int k = 0; k < STEP; ++k)
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j)
+          if (k0 + k < a.nsplit) p[k][j] = peer_f32x4(peer(o + min(r0 + j, nrows - 1) * pitch + d, k0 + k));
+    };
+    fetch(0);
+    const bool none = x.x == -INFINITY && x.y == 0.f;
+    float top = x.x;
+#pragma unroll
+    for (int i = 4; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+    float f = none ? 0.f : exp2_approx(x.x - (top == -INFINITY ? 0.f : top)), sum = f * x.y;
+#pragma unroll
+    for (int i = 4; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+    f = none ? 0.f : f * (a.mask.limit(n, nq, pre, token_of(a, row)) > 0 ? 1.0f / sum : 0.f);
+    const long long at = row_at(a, b, h, row, a.ob, a.ot, a.oh);
+    float v[GROUP][4] = {};
+#pragma unroll 1
+    for (int k0 = 0; k0 < a.nsplit; k0 += STEP) {
+      if (k0 > 0) fetch(k0);
+#pragma unroll
+      for (int k = 0; k < STEP; ++k)
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j) {
+          const float fk = __shfl_sync(0xffffffffu, f, 8 * j + k0 + k);
+          if (k0 + k < a.nsplit) {  // a split without a key for the row may hold anything (fk may be a NaN)
+            const float4 y = fk != 0.f ? p[k][j] : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[j][0] += fk * y.x, v[j][1] += fk * y.y, v[j][2] += fk * y.z, v[j][3] += fk * y.w;
+          }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < GROUP; ++j) {
+      const long long to = __shfl_sync(0xffffffffu, at, 8 * j);
+      if (d < a.dim && r0 + j < nrows) store16x4<HALF>(reinterpret_cast<uint16_t*>(a.out) + to + d, v[j], a.o_wide);
+    }
   }
   cluster_sync();  // no CTA leaves while another may read its memory
 }
@@ -255,7 +287,7 @@ __device__ __forceinline__ int pos_v(int i, int n) {
   return i + LEAD >= n ? n + i : 2 * i + LEAD + 1;
 }
 
-enum { ERR_FULL = 1, ERR_EMPTY, ERR_S, ERR_SFREE, ERR_P, ERR_PV, ERR_Q, ERR_SEEN };
+enum { ERR_FULL = 1, ERR_EMPTY, ERR_S, ERR_SFREE, ERR_P, ERR_PV, ERR_SEEN };
 
 // The producer warp's lane: K and V tiles of one head into the ring, in the order of pos_k and pos_v, places from .. to.
 template <int LEAD, int SLOTS, int MT>
