@@ -62,7 +62,7 @@ fa_status byte_map(CUtensorMap* m, const void* base, uint64_t inner, uint64_t ro
 // The kernel and the splits of whole 128-key tiles: the number of splits with the least time by a model of measured parts (B200, us).
 // A CTA of kv8_attn_few.cu (two on an SM) pays about 4 for its start and end, and for a tile its bytes at the SM's share of the
 // memory (45 GB/s for an SM, 6.5 TB/s for all; lengths are mostly below max_len, hence 0.85). A CTA of kv8_attn_rows.cu (one on an
-// SM) pays about 10, most of it the queries' parts, and 1.9 (fp16 2.1) for a tile. Up to eight splits are a cluster (0.7);
+// SM) pays about 10, its queries' parts and the join of the splits, and 1.9 (fp16 2.1) for a tile. Up to eight splits are a cluster (0.7);
 // more need the merge kernel (3).
 Plan make_plan(const fa_kv8* c, int tokens, int q_heads, int max_len, int sms) {
   Plan p;

@@ -12,6 +12,11 @@
 // shared memory in warp order. The order of k inside the matrix instruction is free as long as both
 // operands share it: a lane owns PB bytes of codes (one or two scale blocks) of each of its rows, read
 // with one load a turn ahead, and x's pairs follow the order in which the codes come out of a word.
+//
+// Measured: 16 rows by 28672 x 8192 in fp16 55 us (2.4 TB/s), 8 by 32768 x 2048 in bf16 16.4 us (2.3 TB/s), one by 2560 x 1024
+// 2.4 us. The memory's time for the first two is 20 and 6 us: what bounds them is taking the codes apart, 8 cycles of a scheduler for a
+// pair of bf16 codes and its scale, 2.2 for fp16. Weights through a ring in shared memory, and CTAs that stay for several
+// rows of W, took longer than registers loaded a turn ahead.
 #include "fa_kv8.cuh"
 
 namespace {
