@@ -513,3 +513,34 @@ def test_quantised_layer_step(require_gpu):
         y = lin(o.view(B, H * D), "o")
         check_linear(y, o.view(B, H * D), *w["o"])
         h = h + y
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,dim", [(1, 256), (2, 128), (20, 64), (20, 256), (150, 128)])
+def test_padding_of_any_content_and_in_place(tokens, dim):
+    """Query rows behind q_lens may hold NaN and infinities, and the output may be the queries: the same bits, and the padding
+    as it was."""
+    c = _filled(2, 1, dim, 300, tokens)
+    lens = torch.tensor([300, 7 + tokens], dtype=torch.int32, device="cuda")
+    qn = torch.tensor([(tokens + 1) // 2, tokens], dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(tokens)
+    q = torch.randn(2, tokens, 4, dim, generator=g).to(BF).cuda()
+    want = c.attend(0, q, lens=lens, q_lens=qn)
+    bad = q.clone()
+    bad[0, (tokens + 1) // 2:, ::2] = float("nan")
+    bad[0, (tokens + 1) // 2:, 1::2] = float("inf")
+    before = bad.clone()
+    c.attend(0, bad, lens=lens, q_lens=qn, out=bad)
+    real = (tokens + 1) // 2
+    assert torch.equal(bad[0, :real], want[0, :real]) and torch.equal(bad[1], want[1])
+    assert torch.equal(bad[0, real:].view(torch.int16), before[0, real:].view(torch.int16))
+
+
+def _filled(batch, heads, dim, n, seed):
+    from flashact_b200 import Kv8Cache
+    c = Kv8Cache(batch, 1, heads, dim, 512)
+    g = torch.Generator().manual_seed(100 + seed)
+    k, v = (torch.randn(batch, n, heads, dim, generator=g).to(BF).cuda() for _ in range(2))
+    c.append(0, k, v)
+    c.advance(n)
+    return c
