@@ -14,9 +14,10 @@
 // with one load a turn ahead, and x's pairs follow the order in which the codes come out of a word.
 //
 // Measured: 16 rows by 28672 x 8192 in fp16 55 us (2.4 TB/s), 8 by 32768 x 2048 in bf16 16.4 us (2.3 TB/s), one by 2560 x 1024
-// 2.4 us. The memory's time for the first two is 20 and 6 us: what bounds them is taking the codes apart, 8 cycles of a scheduler for a
-// pair of bf16 codes and its scale, 2.2 for fp16. Weights through a ring in shared memory, and CTAs that stay for several
-// rows of W, took longer than registers loaded a turn ahead.
+// 2.4 us. The memory's time for the first two is 20 and 6 us. What bounds them is taking the codes apart (8 cycles of a scheduler for
+// a pair of bf16 codes, 2.2 for fp16) with the registers of two warps to a scheduler: of the cycles in which a CTA is there,
+// 44% issue, the rest waits for loads and for results; and the last wave (448 CTAs at 296 places in the first case).
+// Weights through a ring in shared memory, and CTAs that stay for several rows of W, took longer than registers loaded a turn ahead.
 #include "fa_kv8.cuh"
 
 namespace {
