@@ -7,14 +7,17 @@
 // that a part costs no further pass over the cache:
 //   queries  E4M3 parts in units 1, 1/16 (1/256 for fp16), a row scaled by a power of two to [128, 256): bf16 rows are
 //            exact down to 2^-21 of their largest element, fp16 rows to 2^-25;
-//   P        E5M2 parts in units 1, 1/8, 1/64 (1/512 for fp16) of p * 2^12 * vs / (the split's largest vs) rounded to f16:
-//            2^-10 of each p (fp16: 2^-11), its smallest 2^-36: E5M2's range keeps what thousands of faint keys add up to
-//            next to one loud key.
-// The block scales ks, vs multiply scores and probabilities: a thread of the softmax is a key, and has one of each.
+//   P        E5M2 parts in units 1, 1/8, 1/64 (1/512 for fp16) of p_j vs_j 2^12 / 2^d rounded to f16: off by 2^-9 + 2^-11 of a product's
+//            leading power of two (fp16: 2^-11) and by 2^-33 of the row's largest: E5M2's range keeps what thousands of faint keys add up
+//            to next to one loud key.
+// The block scales ks, vs multiply scores and probabilities: a thread of the softmax is a key, and has one of each. 2^d is a power of two
+// of the row's own, near its largest p_j vs_j so far: what a row loses goes by the keys that it sees and their weights, not by the V scales
+// of a block that is masked or has no weight.
 //
 // One CTA takes R query rows of a (observation, key head) and a split of the keys in tiles of 128: warp 0 keeps a ring
 // of K and V tiles full, warp 1 issues the products (scores of tile i + 1 before P V of tile i), warps 2..5 turn scores into
-// probabilities. The running maximum moves only where it grew by more than 2^3, the only case that touches O^T.
+// probabilities. The running maxima (of p and of p vs) move
+// only where one of them grew by more than 2^3, the only case that touches O^T.
 //
 // Bound by the cache's bytes where it is long: one token of 8 observations at 32768 keys of 8 key heads of 128 takes 88 us,
 // 6.1 TB/s. A short cache is a chain of latencies: one observation, 968 keys of one key head of 256, takes 8.2 us (launch 2,
@@ -29,8 +32,8 @@ using namespace fa;
 using namespace fa::kv8;
 
 constexpr int THREADS = 192;
-constexpr float kPTop = 4096.0f;  // p = 1; with a maximum that lags by up to kLag, 2^15 (E5M2 ends at 57344)
-constexpr float kLag = 3.0f;
+constexpr float kPTop = 12.0f;  // log2 of P where p vs = 2^d; with a maximum that lags by up to kLag and kSlack, 2^15.25 (E5M2 ends at 57344)
+constexpr float kLag = 3.0f, kSlack = 0.25f;
 
 __device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
@@ -50,7 +53,7 @@ struct Cfg {
   static constexpr int SLOTS = ((CTAS == 2 ? 113 : 227) * 1024 - REST) / SLOT;
   static constexpr int SMEM = REST + SLOTS * SLOT;
   static_assert(SLOTS >= 3 && SLOTS <= 16 && R % 8 == 0 && R <= 16 && 2 * NS + MT * NP <= 512, "shared or tensor memory");
-  static_assert(SLOTS * 16 + 128 <= 480 && 512 + R * 8 + R * 16 + 16 + 32 + R * 8 <= STATE && R * MT * 512 <= SLOTS * SLOT, "state");
+  static_assert(SLOTS * 16 + 128 <= 480 && 512 + R * 8 + R * 32 + 32 + R * 8 <= STATE && R * MT * 512 <= SLOTS * SLOT, "state");
 };
 
 template <int R, bool HALF, int MT>
@@ -75,9 +78,8 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
   uint64_t* maxes = reinterpret_cast<uint64_t*>(state + 480);  // the four warps' maxima are in wmax
   float* rowscale = reinterpret_cast<float*>(state + 512);     // [R]
   int* rowlim = reinterpret_cast<int*>(rowscale + R);          // [R]
-  float* wmax = reinterpret_cast<float*>(rowlim + R);          // [4][R]
-  float* red = wmax + 4 * R;                                   // [4]
-  int* flags = reinterpret_cast<int*>(red + 4);                // [2][4] a warp of the softmax saw a larger maximum
+  float* wmax = reinterpret_cast<float*>(rowlim + R);          // [4][2][R] of a warp's scores, of its scores and log2 vs
+  int* flags = reinterpret_cast<int*>(wmax + 8 * R);           // [2][4] a warp of the softmax saw a larger maximum
   float2* mls = reinterpret_cast<float2*>(flags + 8);          // [R] maximum and sum of the split, for the cluster
   float* osum = reinterpret_cast<float*>(ring);                // [R][PITCH] and its sums, once the ring is done
   constexpr int PITCH = MT * 128;
@@ -139,16 +141,14 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
     tmem_alloc(tmem_ptr, C::COLS);
     tmem_relinquish();
   }
-  // scales of this thread's key in the first tile, and the largest V scale of the split
-  float k_first = 0.f, v_first = 0.f, vref = 0.f;
+  // scales of this thread's key in the first tile
+  float k_first = 0.f, v_first = 0.f;
   if (w >= 2) {
     const int key = t0 * TILE + key_lane;
     if (key < top) {
       k_first = ldg_now(ks + (key >> a.block_log2));
       v_first = ldg_now(vs + (key >> a.block_log2));
     }
-    const int kend = min(top, (t0 + nt) * TILE);
-    for (int i = ((t0 * TILE) >> a.block_log2) + st; (i << a.block_log2) < kend; i += 128) vref = fmaxf(vref, vs[i]);
     // queries: limits, power-of-two row scales, E4M3 parts; rows behind the last are zero
 #pragma unroll
     for (int j = 0; j < RW; ++j) {
@@ -186,8 +186,6 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
       for (int j = st; j < (C::NP - C::PP * R) * 8; j += 128)
         *reinterpret_cast<uint4*>(ps + i * C::PBYTES + C::PP * R * 128 + j * 16) = make_uint4(0, 0, 0, 0);
     fence_proxy_async_shared();
-    vref = warp_max(vref);
-    if (lane == 0) red[quad] = vref;
   }
   tc_fence_before();
   __syncthreads();
@@ -236,12 +234,10 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
     }
   } else {
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    vref = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float vinv = vref > 0.f ? kPTop / vref : 0.f;
-
-    float m[R], l[R], rs[R];  // the subtracted maximum (the same in all threads), this key lane's sum, the rows' scales
+    // The subtracted maximum and the exponent d of p vs, a whole number (both the same in all threads), this key lane's sum.
+    float m[R], d[R], l[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) m[r] = -INFINITY, l[r] = 0.f, rs[r] = rowscale[r];
+    for (int r = 0; r < R; ++r) m[r] = -INFINITY, d[r] = 0.f, l[r] = 0.f;
     float kn = k_first, vn = v_first;
     int grown = 0;  // times that the maximum moved
     auto scales = [&](int i) {
@@ -253,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
     bool ok = true;
     for (int i = 0; i < nt; ++i) {
       const int key = (t0 + i) * TILE + key_lane;
-      const float kscale = kn, vfac = vn * vinv;
+      const float kscale = kn, lv = log2_approx(vn);
       scales(i + 1);
       ok = mbar_wait(sfull + (i & 1), (i >> 1) & 1, err, ERR_S);
       ok = __all_sync(0xffffffffu, ok);
@@ -276,14 +272,17 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
         }
       }
 #pragma unroll
-      for (int r = 0; r < R; ++r) s[r] *= rs[r] * kscale;
+      for (int r = 0; r < R; ++r) s[r] *= rowscale[r] * kscale;
       if ((t0 + i) * TILE + TILE > low) {  // not seen by every row
 #pragma unroll
         for (int r = 0; r < R; ++r) s[r] = key < rowlim[r] ? s[r] : -INFINITY;
       }
       bool grew = false;
 #pragma unroll
-      for (int r = 0; r < R; ++r) grew |= s[r] > m[r] + kLag;
+      for (int r = 0; r < R; ++r) {
+        const float t = s[r] - m[r];
+        grew |= t > kLag || t + lv > d[r] + kLag;
+      }
       grew = __any_sync(0xffffffffu, grew);
       if (lane == 0) {
         flags[(i & 1) * 4 + quad] = grew;
@@ -294,23 +293,36 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
       if (!ok) break;
       const int4 fl = *reinterpret_cast<const int4*>(flags + (i & 1) * 4);
       if (fl.x | fl.y | fl.z | fl.w) {  // the same in all 128 threads
+        float x[2 * R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const float x = warp_max(s[r]);
-          if (lane == 0) wmax[quad * R + r] = x;
+        for (int r = 0; r < R; ++r) x[r] = warp_max(s[r]), x[R + r] = warp_max(s[r] + lv);
+        if (lane == 0) {
+#pragma unroll
+          for (int r = 0; r < 2 * R; r += 4)
+            *reinterpret_cast<float4*>(wmax + quad * 2 * R + r) = make_float4(x[r], x[r + 1], x[r + 2], x[r + 3]);
+          mbar_arrive(maxes);
         }
-        if (lane == 0) mbar_arrive(maxes);
         ok = mbar_wait(maxes, grown & 1, err, ERR_SEEN);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ++grown;
         float f[R];
 #pragma unroll
+        for (int r = 0; r < 2 * R; r += 4) {
+          float4 y[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[k] = *reinterpret_cast<const float4*>(wmax + k * 2 * R + r);
+          x[r] = fmaxf(fmaxf(y[0].x, y[1].x), fmaxf(y[2].x, y[3].x)), x[r + 1] = fmaxf(fmaxf(y[0].y, y[1].y), fmaxf(y[2].y, y[3].y));
+          x[r + 2] = fmaxf(fmaxf(y[0].z, y[1].z), fmaxf(y[2].z, y[3].z)), x[r + 3] = fmaxf(fmaxf(y[0].w, y[1].w), fmaxf(y[2].w, y[3].w));
+        }
+#pragma unroll
         for (int r = 0; r < R; ++r) {
-          const float x = fmaxf(m[r], fmaxf(fmaxf(wmax[r], wmax[R + r]), fmaxf(wmax[2 * R + r], wmax[3 * R + r])));
-          f[r] = x == -INFINITY ? 1.f : exp2_approx(m[r] - x);
-          m[r] = x;
-          l[r] *= f[r];
+          const float mn = fmaxf(m[r], x[r]), nv = fmaxf(m[r] + d[r], x[R + r]);
+          const float down = mn == -INFINITY ? 0.f : m[r] - mn;
+          const float dn = mn == -INFINITY ? 0.f : fminf(fmaxf(ceilf(nv - mn - kSlack), -114.f), 126.f);
+          f[r] = exp2_approx(down + (d[r] - dn));
+          l[r] *= exp2_approx(down);
+          m[r] = mn, d[r] = dn;
         }
         if (i > 0) {
           ok = mbar_wait(pvdone + ((i - 1) & 1), ((i - 1) >> 1) & 1, err, ERR_PV);
@@ -341,11 +353,10 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
       unsigned char* pb = ps + (i & 1) * C::PBYTES;
 #pragma unroll
       for (int r = 0; r < R; r += 2) {
-        const float x = exp2_approx(s[r] - (m[r] == -INFINITY ? 0.f : m[r]));
-        const float y = exp2_approx(s[r + 1] - (m[r + 1] == -INFINITY ? 0.f : m[r + 1]));
-        l[r] += x;
-        l[r + 1] += y;
-        uint32_t p = pack_f16x2(x * vfac, y * vfac);
+        const float x = s[r] - (m[r] == -INFINITY ? 0.f : m[r]), y = s[r + 1] - (m[r + 1] == -INFINITY ? 0.f : m[r + 1]);
+        l[r] += exp2_approx(x);
+        l[r + 1] += exp2_approx(y);
+        uint32_t p = pack_f16x2(exp2_approx(x + (lv + kPTop - d[r])), exp2_approx(y + (lv + kPTop - d[r + 1])));
 #pragma unroll
         for (int k = 0; k < C::PP; ++k) {
           pb[swz(k * R + r, key_lane)] = (unsigned char)(p >> 8);
@@ -384,7 +395,9 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
       for (int k = 0; k < R; ++k) top_m = k == r ? m[k] : top_m;
       if (lane == 0) mls[r] = make_float2(top_m, x);
     }
-    const float unit = vref * (1.0f / kPTop);
+    float unit[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) unit[r] = __int_as_float(((int)d[r] - (int)kPTop + 127) << 23);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       float v[C::NP];
@@ -398,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
           if (r >= nrows) break;
           float x = v[r] + v[R + r] * 0.125f + v[2 * R + r] * (1.0f / 64.0f);
           if (HALF) x += v[(C::PP - 1) * R + r] * (1.0f / 512.0f);
-          x = ok ? x * unit : __int_as_float(0x7fffffff);  // a wait that ran out is seen in the result
+          x = ok ? x * unit[r] : __int_as_float(0x7fffffff);  // a wait that ran out is seen in the result
           osum[r * PITCH + d] = x;
         }
       }

@@ -6,8 +6,9 @@
 // sums of 8-bit parts, each the rounding of what the parts before it left over, and every part is one more product into the same sums:
 //   queries  two E4M3 parts (three for fp16) of a row scaled by a power of two to [128, 256): off by at most 2^-10, that is 2^-17 of
 //            the row's largest element, where E4M3's smallest steps end it;
-//   P        three E5M2 parts (four for fp16) of p * 2^14 * vs / (the split's largest vs) rounded to f16: 2^-10 of each p
-//            (fp16: 2^-11) and no less than 2^-31 of the largest.
+//   P        three E5M2 parts (four for fp16) of p_j vs_j 2^14 / 2^d rounded to f16: off by 2^-9 + 2^-11 of a product's leading power of two
+//            (fp16: 2^-11) and by 2^-29 of the row's largest. 2^d is the row's own, near its largest p_j vs_j so far: what a row loses goes by
+//            the keys that it sees and their weights, not by the V scales of a block that is masked or has no weight.
 // That is 2 + 3 products at the 8-bit rate against the 2 + 2 that one bf16 product each would cost at half that rate,
 // without converting the cache or holding it in 16 bits in shared memory, whose bandwidth would bound it.
 //
@@ -16,8 +17,8 @@
 //
 // Warp 0 keeps a ring of K and V tiles (128 keys) full, warp 1 issues the scores' products (up to two tiles ahead), warp 2
 // those of P and V, warps 4..11 turn scores into probabilities: a thread has one query row and half of the tile's keys, and
-// the two threads of a row exchange their maxima, those of tile i + 1 while they write P of tile i. The running maximum
-// moves only where it grew by more than 2^1, the only case that touches O.
+// the two threads of a row exchange their maxima, those of tile i + 1 while they write P of tile i. The running maxima (of p and of
+// p vs) move only where one of them grew by more than 2^1, the only case that touches O.
 //
 // Measured at head_dim 256 (bf16): a tile takes about 2 us, its products 2560 cycles of that (64 for a score product of K = 32,
 // 128 for one of P V); a CTA's start 4 us, 2 of them the queries' parts, its end 5. 16 observations of 50 tokens and 8
@@ -33,8 +34,8 @@ using namespace fa;
 using namespace fa::kv8;
 
 constexpr int THREADS = 384, ROWS = 128, SOFT = 4;  // SOFT: first softmax warp
-constexpr float kPTop = 16384.0f;  // p = 1; with a maximum that lags by up to kLag, 2^15 (E5M2 ends at 57344)
-constexpr float kLag = 1.0f;
+constexpr float kPTop = 14.0f;  // log2 of P where p vs = 2^d; with a maximum that lags by up to kLag and kSlack, 2^15.25 (E5M2 ends at 57344)
+constexpr float kLag = 1.0f, kSlack = 0.25f;
 
 template <bool HALF, int MT_>
 struct Cfg {
@@ -67,8 +68,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* seen = pvdone + 1;                          // the eight warps' maxima are in half_max
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(seen + 1);
   volatile int* err = reinterpret_cast<volatile int*>(tmem_ptr + 1);
-  float* red = reinterpret_cast<float*>(state + 256);       // [8]
   float* half_max = reinterpret_cast<float*>(state + 512);  // [2][2][128], a tile's maxima in the one of its parity
+  signed char* half_exp = reinterpret_cast<signed char*>(state + 2560);  // [2][2][128], the exponent of p vs above each of them
   float* rowscale = half_max + 2 * ROWS;                    // [128], read before the second tile's maxima
   float* osum = reinterpret_cast<float*>(smem);             // [128][PITCH] sums of the split and, behind a row, its maximum and sum
   constexpr int PITCH = MT * 128 + 4;
@@ -113,7 +114,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     tmem_alloc(tmem_ptr, 512);
     tmem_relinquish();
   }
-  float vref = 0.f;  // largest V scale of the split
   if (w >= SOFT) {
     // queries: power-of-two row scales and E4M3 parts; rows behind the last are zero
     constexpr int LANES = MT * 16, PER = 32 / LANES, N = 16 / PER;  // lanes of a row, rows at a time, such groups of the warp's 16 rows
@@ -182,8 +182,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         *reinterpret_cast<uint2*>(dst + p * MT * 16384) = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
       }
     };
-    const int kend = min(top, (t0 + nt) * TILE);
-    for (int i = ((t0 * TILE) >> a.block_log2) + tid - SOFT * 32; (i << a.block_log2) < kend; i += 256) vref = fmaxf(vref, vs[i]);
     cp_async_wait_all();
     __syncwarp();
 #pragma unroll 1
@@ -208,8 +206,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int j = 0; j < 4; ++j) split(j0 + j, q[j], m[j]);
     }
     fence_proxy_async_shared();
-    vref = warp_max(vref);
-    if (lane == 0) red[w - SOFT] = vref;
   }
   tc_fence_before();
   __syncthreads();
@@ -262,9 +258,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else if (w >= SOFT) {
     const int half = (w - SOFT) >> 2, quad = w & 3, row = quad * 32 + lane, st = tid - SOFT * 32;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) vref = fmaxf(vref, red[i]);
-    const float vinv = vref > 0.f ? kPTop / vref : 0.f;
     const float rs = rowscale[row];
     const int lim = row < nrows ? a.mask.limit(n, nq, pre, token_of(a, row0 + row)) : 0;
 
@@ -274,11 +267,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       next = lane < 8 && i < nt && key < top ? __ldg((lane < 4 ? ks : vs) + (key >> a.block_log2)) : 0.f;
     };
     scales(0);
-    float m = -INFINITY, l = 0.f;  // the subtracted maximum (the same in a row's two threads), this half's sum
+    // the subtracted maximum and the exponent of p vs (both the same in a row's two threads), this half's sum
+    float m = -INFINITY, d = 0.f, l = 0.f;
     bool ok = true;
     // Raw scores s of a tile, factors f per 16-key group (the scale's sign went into the queries, so f >= 0 and a group's maximum
-    // is f times that of its scores), and this half's maximum on its way to the row's other thread. Masked scores are -inf.
-    float s[64], f[4], vf[4], mx;
+    // is f times that of its scores), log2 of the groups' V scales, and this half's maximum and the exponent above it (whole, so that it
+    // goes through a byte) on their way to the row's other thread. Masked scores are -inf.
+    float s[64], f[4], lv[4], mx, mv;
     auto fetch = [&](int i) {
       ok = mbar_wait(sfull, i & 1, err, ERR_S);
       ok = __all_sync(0xffffffffu, ok);
@@ -290,10 +285,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(sfree);
+      const float next_log = log2_approx(next);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         f[j] = rs * __shfl_sync(0xffffffffu, next, j);
-        vf[j] = __shfl_sync(0xffffffffu, next, 4 + j) * vinv;
+        lv[j] = __shfl_sync(0xffffffffu, next_log, 4 + j);
       }
       if ((t0 + i) * TILE + TILE > low) {  // not seen by every row
         const int left = lim - (t0 + i) * TILE - half * 64;
@@ -303,15 +299,20 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int j = 0; j < 4; ++j) f[j] = f[j] == 0.f ? 1e-30f : f[j];  // -inf stays -inf
       }
       scales(i + 1);
-      mx = -INFINITY;
+      mx = -INFINITY, mv = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float g = s[16 * j];
 #pragma unroll
         for (int c = 1; c < 15; c += 2) g = max3(g, s[16 * j + c], s[16 * j + c + 1]);
-        mx = fmaxf(mx, fmaxf(g, s[16 * j + 15]) * f[j]);
+        g = fmaxf(g, s[16 * j + 15]) * f[j];
+        mx = fmaxf(mx, g);
+        mv = fmaxf(mv, g + lv[j]);
       }
+      const float up = mx == -INFINITY ? 0.f : fminf(fmaxf(ceilf(mv - mx - kSlack), -126.f), 126.f);
+      mv = mx + up;
       half_max[(i & 1) * 2 * ROWS + half * ROWS + row] = mx;
+      half_exp[(i & 1) * 2 * ROWS + half * ROWS + row] = (signed char)up;
       __syncwarp();
       if (lane == 0) mbar_arrive(seen);
     };
@@ -320,12 +321,17 @@ __global__ void __launch_bounds__(THREADS, 1)
       ok = mbar_wait(seen, i & 1, err, ERR_SEEN);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      mx = fmaxf(mx, half_max[(i & 1) * 2 * ROWS + (half ^ 1) * ROWS + row]);
-      const bool grew = mx > m + kLag || (m == -INFINITY && mx > m);
+      {
+        const int other = (i & 1) * 2 * ROWS + (half ^ 1) * ROWS + row;
+        mv = fmaxf(mv, half_max[other] + (float)half_exp[other]);
+        mx = fmaxf(mx, half_max[other]);
+      }
+      const bool grew = mx > m + kLag || mv > m + d + kLag || (m == -INFINITY && mx > m);
       if (__any_sync(0xffffffffu, grew)) {  // the same in the row's other thread's warp
-        const float x = fmaxf(m, mx), down = x == -INFINITY ? 1.f : exp2_approx(m - x);
-        m = x;
-        l *= down;
+        const float x = fmaxf(m, mx), by = x == -INFINITY ? 0.f : m - x;
+        const float dn = x == -INFINITY ? 0.f : fmaxf(fmaxf(m + d, mv) - x, -110.f), down = exp2_approx(by + (d - dn));
+        l *= exp2_approx(by);
+        m = x, d = dn;
         if (i > 0) {  // O is at rest once the tile before is done
           ok = mbar_wait(pvdone, (i - 1) & 1, err, ERR_PV);
           ok = __all_sync(0xffffffffu, ok);
@@ -348,10 +354,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t e[C::PP][16];  // all of P before the wait for its place, which the product of the tile before still reads
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        // p vs / vref 2^14 straight from the exponent; the sum of p is that of a group over its factor. A factor below 2^-40 counts as
+        // p vs 2^(14 - d) straight from the exponent; the sum of p is that of a group over its factor. A factor below 2^-40 counts as
         // that: such a P is 0 in f16 either way.
-        const float v = vf[j] < 9.094947e-13f ? 9.094947e-13f : vf[j], lv = log2_approx(v);
-        const float cc = lv - base;
+        float v = lv[j] + (kPTop - d);
+        v = v < -40.f ? -40.f : v;
+        const float cc = v - base;
         float g0 = 0.f, g1 = 0.f;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -368,7 +375,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (k + 1 < C::PP) p = rest1(p), q = rest1(q);
           }
         }
-        l += (g0 + g1) * exp2_approx(-lv);
+        l += (g0 + g1) * exp2_approx(-v);
       }
       if (i + 1 < nt) fetch(i + 1);
       if (!ok) break;
@@ -401,7 +408,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     bar_softmax();
     l = sums[row] + sums[ROWS + row];
     if (half == 0) *reinterpret_cast<float2*>(osum + row * PITCH + MT * 128) = make_float2(m, l);
-    const float norm = ok ? vref * (1.0f / kPTop) : __int_as_float(0x7fffffff);  // a wait that ran out is seen in the result
+    const float norm = ok ? exp2_approx(d - kPTop) : __int_as_float(0x7fffffff);  // a wait that ran out is seen in the result
 #pragma unroll 1
     for (int c = half * 32; c < a.dim; c += 64) {
       float v[32];
