@@ -7,9 +7,9 @@
 // that a part costs no further pass over the cache:
 //   queries  E4M3 parts in units 1, 1/16 (1/256 for fp16), a row scaled by a power of two to [128, 256): bf16 rows are
 //            exact down to 2^-21 of their largest element, fp16 rows to 2^-25;
-//   P        E5M2 parts in units 1, 1/8, 1/64 (1/512 for fp16) of p_j vs_j 2^12 / 2^d rounded to f16: off by 2^-9 + 2^-11 of a product's
-//            leading power of two (fp16: 2^-11) and by 2^-33 of the row's largest: E5M2's range keeps what thousands of faint keys add up
-//            to next to one loud key.
+//   P        E5M2 parts of p_j vs_j 2^12 / 2^d: three in units 1, 1/8, 1/64 hold what f16 holds of it, 2^-11 of a product's leading power of
+//            two; for fp16 a fourth in units of 1/512 holds what f16 lost, 2^-15. All end at 2^-33 of the row's largest product: E5M2's range
+//            keeps what thousands of faint keys add up to next to one loud key.
 // The block scales ks, vs multiply scores and probabilities: a thread of the softmax is a key, and has one of each. 2^d is a power of two
 // of the row's own, near its largest p_j vs_j so far: what a row loses goes by the keys that it sees and their weights, not by the V scales
 // of a block that is masked or has no weight.
@@ -356,13 +356,15 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
         const float x = s[r] - (m[r] == -INFINITY ? 0.f : m[r]), y = s[r + 1] - (m[r + 1] == -INFINITY ? 0.f : m[r + 1]);
         l[r] += exp2_approx(x);
         l[r + 1] += exp2_approx(y);
-        uint32_t p = pack_f16x2(exp2_approx(x + (lv + kPTop - d[r])), exp2_approx(y + (lv + kPTop - d[r + 1])));
+        const float px = exp2_approx(x + (lv + kPTop - d[r])), py = exp2_approx(y + (lv + kPTop - d[r + 1]));
+        uint32_t p = pack_f16x2(px, py);
+        [[maybe_unused]] const uint32_t lost = HALF ? __byte_perm(f16_lost(px, py, p, 512.f), 0, 0x1404) : 0u;
 #pragma unroll
         for (int k = 0; k < C::PP; ++k) {
-          pb[swz(k * R + r, key_lane)] = (unsigned char)(p >> 8);
-          pb[swz(k * R + r + 1, key_lane)] = (unsigned char)(p >> 24);
-          if (k + 1 < C::PP) p = rest8(p);
-          if (!HALF && k + 2 == C::PP) p = round_part(p);
+          const uint32_t e = k < 3 ? round_part(p) : lost;
+          pb[swz(k * R + r, key_lane)] = (unsigned char)(e >> 8);
+          pb[swz(k * R + r + 1, key_lane)] = (unsigned char)(e >> 24);
+          if (k < 2) p = rest8(p, e);
         }
       }
       const int left = top - (t0 + i) * TILE;

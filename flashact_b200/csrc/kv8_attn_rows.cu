@@ -6,9 +6,10 @@
 // sums of 8-bit parts, each the rounding of what the parts before it left over, and every part is one more product into the same sums:
 //   queries  two E4M3 parts (three for fp16) of a row scaled by a power of two to [128, 256): off by at most 2^-10, that is 2^-17 of
 //            the row's largest element, where E4M3's smallest steps end it;
-//   P        three E5M2 parts (four for fp16) of p_j vs_j 2^14 / 2^d rounded to f16: off by 2^-9 + 2^-11 of a product's leading power of two
-//            (fp16: 2^-11) and by 2^-29 of the row's largest. 2^d is the row's own, near its largest p_j vs_j so far: what a row loses goes by
-//            the keys that it sees and their weights, not by the V scales of a block that is masked or has no weight.
+//   P        E5M2 parts of p_j vs_j 2^14 / 2^d: three hold what f16 holds of it, 2^-11 of a product's leading power of two; for fp16 a
+//            fourth holds what f16 lost, 2^-15. They end at 2^-29 of the row's largest product. 2^d is the row's own, near its largest p_j vs_j
+//            so far: what a row loses goes by the keys that it sees and their weights, not by the V scales of a block that is masked or has no
+//            weight. fp16 without the fourth part took 65.4 us instead of 76.2 (256 tokens, below), 1.3 times the plain form's error instead of 1.0.
 // That is 2 + 3 products at the 8-bit rate against the 2 + 2 that one bf16 product each would cost at half that rate,
 // without converting the cache or holding it in 16 bits in shared memory, whose bandwidth would bound it.
 //
@@ -23,7 +24,7 @@
 // Measured at head_dim 256 (bf16): a tile takes about 2 us, its products 2560 cycles of that (64 for a score product of K = 32,
 // 128 for one of P V); a CTA's start 4 us, 2 of them the queries' parts, its end 5. 16 observations of 50 tokens and 8
 // query heads on one key head at 1018 keys: 26 us (258 TFLOP/s, each product counted once); 4 of 256 tokens in fp16 at up to
-// 4096: 71 us (389). With 16-bit products and converted tiles these took 74 and 222 us. Rows come here from 17 on: a tile of
+// 4096: 76 us (364). With 16-bit products and converted tiles these took 74 and 222 us. Rows come here from 17 on: a tile of
 // 128 costs the same however many of its rows are used, and kv8_attn_few.cu needs tensor memory columns for each part of
 // each row, enough for 16.
 #include "kv8_tc.cuh"
@@ -368,11 +369,12 @@ __global__ void __launch_bounds__(THREADS, 1)
           g0 += x0 + x1;
           g1 += x2 + x3;
           uint32_t p = pack_f16x2(x0, x1), q = pack_f16x2(x2, x3);
+          if (HALF) e[C::PP - 1][4 * j + c] = __byte_perm(f16_lost(x0, x1, p, 1.f), f16_lost(x2, x3, q, 1.f), 0x5410);
 #pragma unroll
-          for (int k = 0; k < C::PP; ++k) {
-            if (!HALF && k + 1 == C::PP) p = round_part(p), q = round_part(q);
-            e[k][4 * j + c] = __byte_perm(p, q, 0x7531);  // the upper bytes
-            if (k + 1 < C::PP) p = rest1(p), q = rest1(q);
+          for (int k = 0; k < 3; ++k) {
+            const uint32_t pr = round_part(p), qr = round_part(q);
+            e[k][4 * j + c] = __byte_perm(pr, qr, 0x7531);  // the upper bytes
+            if (k < 2) p = rest1(p, pr), q = rest1(q, qr);
           }
         }
         l += (g0 + g1) * exp2_approx(-v);

@@ -63,19 +63,28 @@ __device__ __forceinline__ uint32_t f32x2_e4m3x2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// E5M2 is f16's upper byte: cutting a non-negative f16 there leaves its first three significant bits, and what was cut off is
-// again an f16. Four such parts hold all its eleven bits; of three, the last is rounded instead of cut (p is at most 2^15, so
-// that no carry leaves a half).
+// E5M2 is f16's upper byte: rounding an f16 there (half up in magnitude; |p| is below 57344, so that no carry makes an infinity) leaves
+// three significant bits, and what it leaves over, of either sign, is again an f16 and at most 2^-3 of the leading power of two. Three such parts
+// are 3 + 4 + 4 bits: all eleven of an f16 (cut instead of rounded they would hold nine).
 __device__ __forceinline__ uint32_t round_part(uint32_t p) { return p + 0x00800080u; }
-__device__ __forceinline__ uint32_t rest1(uint32_t p) {
-  const uint32_t v = p & 0xff00ff00u;
+__device__ __forceinline__ uint32_t rest1(uint32_t p, uint32_t rounded) {
+  const uint32_t v = rounded & 0xff00ff00u;
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&p), *reinterpret_cast<const __half2*>(&v));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t rest8(uint32_t p) {  // eight times that: at most 2^15 where p was
-  const uint32_t d = rest1(p);
+__device__ __forceinline__ uint32_t rest8(uint32_t p, uint32_t rounded) {  // eight times that: at most 2^15.25 where p was
+  const uint32_t d = rest1(p, rounded);
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&d), __float2half2_rn(8.f));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+// What the rounding of x, y to the f16 pair p left over, times `up`, in E5M2 (the lower byte is x's).
+__device__ __forceinline__ uint32_t f16_lost(float x, float y, uint32_t p, float up) {
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&p));
+  uint16_t r;
+  asm("{\n\t.reg .b64 v, n, m;\n\t.reg .f32 a, b;\n\tmov.b64 v, {%1, %2};\n\tmov.b64 n, {%3, %4};\n\t"
+      "mov.b64 m, {%5, %5};\n\tfma.rn.f32x2 v, n, m, v;\n\tmov.b64 {a, b}, v;\n\t"
+      "cvt.rn.satfinite.e5m2x2.f32 %0, b, a;\n\t}" : "=h"(r) : "f"(x * up), "f"(y * up), "f"(h.x), "f"(h.y), "f"(-up));
+  return r;
 }
 __device__ __forceinline__ uint32_t f16x2_e4m3x2(uint32_t v) {
   uint16_t r;

@@ -3,13 +3,14 @@ import torch
 
 from tests.kv8_util import values
 
-# Bits that the kernels keep of a probability times its V scale, and where they end, relative to the largest such product of the row.
-#   p_rel: half a step of what the parts hold, relative to the product's leading power of two.
-#   p_abs: few rows: P holds the row's largest product at 2^11.25 or more, and its smallest steps (f16's 2^-24, and the last part's
-#          2^-16 in units of 1/64 or 1/512) lose 2^-25 + 2^-23 at most: below 2^-33 of the largest. More rows: the largest at 2^13.25 or more,
-#          all parts in units of 1, half a step of 2^-16 and f16's 2^-25: below 2^-30 + 2^-38, under 2^-29.
-P_REL = {(True, torch.bfloat16): 2.0 ** -9 + 2.0 ** -11, (True, torch.float16): 2.0 ** -11,
-         (False, torch.bfloat16): 2.0 ** -9 + 2.0 ** -11, (False, torch.float16): 2.0 ** -11}
+# Bits that the kernels keep of a probability times its V scale, and where they end, relative to the largest such product of the row
+# (tests/test_kv8_values.py goes through the parts on the CPU).
+#   P_REL: f16 holds eleven bits, and three E5M2 parts rounded to nearest hold all of them: half a step, 2^-11 of the product's leading power of
+#          two. fp16 queries have a fourth part for what f16 lost, at most 2^-11, rounded to three bits: 2^-15.
+#   p_abs: few rows: P holds the row's largest product at 2^11.25 or more; the third part's smallest step is 2^-16 / 64, the fourth's
+#          2^-16 / 512, f16's own 2^-24; half of each: below 2^-22.6, under 2^-33 of the largest. More rows: the largest at 2^13.25 or more,
+#          all parts in units of 1, half a step of 2^-16 for the third and for the fourth, f16's 2^-25: under 2^-29 of the largest.
+P_REL = {torch.bfloat16: 2.0 ** -11, torch.float16: 2.0 ** -15}
 
 
 def seen_by(lens, T, causal, prefix, q_lens):
@@ -22,10 +23,10 @@ def seen_by(lens, T, causal, prefix, q_lens):
     return out
 
 
-def attend(ref, layer, q, lens, *, causal=True, prefix=None, q_lens=None, scale=None, p_rel=None):
+def attend(ref, layer, q, lens, *, causal=True, prefix=None, q_lens=None, scale=None):
     """(out, tol), both [B][T][H][D]; softmax(scale q K^T + mask) V of the cache `ref` (tests/kv8_util.py).
 
-    The tolerance counts roundings, for each row by the keys that it sees alone. Output: half a step of q's type. Products p_j vs_j: p_rel and
+    The tolerance counts roundings, for each row by the keys that it sees alone. Output: half a step of q's type. Products p_j vs_j: P_REL and
     p_abs above. Scores: fp32 sums of D products off by (D + 8) 2^-23 of scale sum |q k| (the matrix unit truncates), queries given in parts off
     by 2^-17 of the row's largest element (few rows 2^-21), the exponential and the scales' logarithm by 2^-20 together: a share of p
     in numerator and sum."""
@@ -35,7 +36,7 @@ def attend(ref, layer, q, lens, *, causal=True, prefix=None, q_lens=None, scale=
     group = H // heads
     scale = D ** -0.5 if scale is None else scale
     few = T * group <= 16
-    p_rel = P_REL[few, q.dtype] if p_rel is None else p_rel
+    p_rel = P_REL[q.dtype]
     p_abs, low_q = (2.0 ** -33, 2.0 ** -21) if few else (2.0 ** -29, 2.0 ** -17)
     u = torch.finfo(q.dtype).eps / 2
     see = seen_by(lens, T, causal, prefix, q_lens)

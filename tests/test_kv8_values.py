@@ -1,8 +1,9 @@
 """Attention over the 8-bit KV cache: what a row's result may depend on, and how many bits it keeps."""
+import numpy as np
 import pytest
 import torch
 
-from tests.kv8_bounds import attend, check
+from tests.kv8_bounds import P_REL, attend, check
 from tests.kv8_util import random_ref
 
 BF, HF = torch.bfloat16, torch.float16
@@ -10,6 +11,51 @@ BF, HF = torch.bfloat16, torch.float16
 
 def _q(shape, dtype, seed):
     return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def _e5m2(x):
+    """The nearest E5M2 value (half up in magnitude) of f16 numbers, by their bits: the upper byte of an f16."""
+    return ((x.view(np.uint16) + np.uint16(0x80)) & np.uint16(0xFF00)).view(np.float16)
+
+
+@pytest.mark.parametrize("up", [1.0, 8.0])
+def test_three_rounded_parts_hold_an_f16(up):
+    """Every f16 up to 2^15.25: three E5M2 parts, each the rounding of what the parts before it left over (times `up` a part), are its value
+    but for the last part's smallest steps; no part leaves the type; cut parts would lose two bits."""
+    p = np.arange(1, 0x7C00, dtype=np.uint16).view(np.float16)
+    p = p[p.astype(np.float64) <= 2.0 ** 15.25]
+    rest, total, unit = p, np.zeros(p.shape), 1.0
+    for _ in range(3):
+        part = _e5m2(rest)
+        assert np.isfinite(part).all() and np.abs(part.astype(np.float64)).max() <= 57344
+        total += part.astype(np.float64) * unit
+        left = rest.astype(np.float64) - part.astype(np.float64)
+        rest, unit = (left * up).astype(np.float16), unit / up
+        assert (rest.astype(np.float64) == left * up).all()  # the kernel's f16 subtraction loses nothing
+    x = p.astype(np.float64)
+    lost = np.abs(total - x)
+    assert (lost <= 2.0 ** -17 / up ** 2).all()
+    assert (lost[x >= 2.0 ** (-6 - 2 * np.log2(up))] == 0).all()
+    cut = lambda y: (y.view(np.uint16) & np.uint16(0xFF00)).view(np.float16)  # noqa: E731
+    a = cut(p)
+    b = cut((x - a).astype(np.float16))
+    c = _e5m2((x - a - b).astype(np.float16))
+    big = x >= 1
+    assert np.abs(x - a - b - c)[big].max() > 0 and (np.abs(x - a - b - c) / x)[big].max() > 3 * P_REL[BF]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("T,H,D", [(4, 2, 64), (2, 8, 256), (4, 4, 128), (40, 2, 64), (24, 8, 256), (30, 8, 96)])
+@pytest.mark.parametrize("n", [2, 3, 5, 40])
+def test_probabilities_keep_their_bits(require_gpu, T, H, D, dtype, n):
+    """A few keys of unlike weight whose values have one sign, so that nothing hides behind cancellation: a part of P that went missing
+    is 2^-7 (bf16) or 2^-11 (fp16) of the output."""
+    ref = random_ref(4, 1, 1, D, 64, 16, n)
+    ref.v &= 0x7F
+    q = _q((4, T, H, D), dtype, n)
+    want, tol = attend(ref, 0, q, [n] * 4, causal=False)
+    check(ref.to_cache([n] * 4).attend(0, q.cuda(), causal=False), want, tol)
 
 
 # tokens, query heads of one key head: 8, 16 and more rows
