@@ -17,6 +17,7 @@ EXPORTS = ["fa_create", "fa_pi05_load_weights", "fa_pi05_load_weights_q", "fa_ma
            "fa_sync", "fa_set_stage_timing", "fa_get_stage_cycles", "fa_last_launch_count",
            "fa_set_fault_injection", "fa_debug_trace", "fa_pi05_modulations_noalloc", "fa_quantize_fp8_rows", "fa_quantize_nvfp4",
            "fa_nvfp4_linear", "fa_kv8_append", "fa_kv8_read", "fa_kv8_attention_workspace", "fa_kv8_attention",
+           "fa_kv8_set_fault_injection",
            "fa_last_error", "fa_destroy"]
 
 
@@ -112,6 +113,7 @@ def load_library(path: str = None) -> ctypes.CDLL:
         "fa_kv8_read": (S, [KV, P, I, P, P, I, P]),
         "fa_kv8_attention_workspace": (S, [KV, I, I, I, ctypes.POINTER(ctypes.c_size_t)]),
         "fa_kv8_attention": (S, [KV, I, I, I, R, I, P, P, P, I, ctypes.c_float, I, R, P, ctypes.c_size_t, P]),
+        "fa_kv8_set_fault_injection": (None, [I, ctypes.c_uint]),
         "fa_last_error": (ctypes.c_char_p, [H]),
         "fa_destroy": (None, [H]),
     }

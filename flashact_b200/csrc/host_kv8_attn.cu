@@ -102,6 +102,9 @@ fa_status attn_check(const fa_kv8* c, int tokens, int q_heads, int max_len) {
   return FA_OK;
 }
 
+std::atomic<int> fault_split{-1};
+std::atomic<unsigned> spin_limit{0};
+
 // SMs of the current device; 148 where there is none, so that a workspace can be sized anywhere.
 int sm_count(int* device = nullptr) {
   static std::atomic<int> known[64];
@@ -121,6 +124,11 @@ int sm_count(int* device = nullptr) {
 }
 
 }  // namespace
+
+extern "C" void fa_kv8_set_fault_injection(int split, unsigned limit) {
+  fault_split.store(split, std::memory_order_relaxed);
+  spin_limit.store(limit, std::memory_order_relaxed);
+}
 
 extern "C" fa_status fa_kv8_attention_workspace(const fa_kv8* c, int tokens, int q_heads, int max_len, size_t* bytes) {
   fa_status st = attn_check(c, tokens, q_heads, max_len);
@@ -160,6 +168,9 @@ extern "C" fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, in
   if (p.part_bytes && (st = check_pointers({{"workspace", workspace}})) != FA_OK) return st;
   AttnArgs a;
   a.device = device;
+  const unsigned limit = spin_limit.load(std::memory_order_relaxed);
+  a.fault_split = fault_split.load(std::memory_order_relaxed);
+  a.spin_limit = limit ? (int)std::min(limit, fa::kSpinLimit) : (int)fa::kSpinLimit;
   a.k = c->k, a.v = c->v, a.ks = c->k_scale, a.vs = c->v_scale;
   a.q = q->ptr, a.out = out->ptr;
   a.qb = q->batch, a.qt = q->token, a.qh = q->head;

@@ -20,6 +20,7 @@ struct AttnArgs {
   // each takes an equal share of the observation's own tiles, else tiles [split * split_chunks, + split_chunks).
   int nsplit, cluster, split_chunks;
   int device;
+  int fault_split, spin_limit;  // test hook: the split whose first scores are never announced (-1: none); polls of a wait
   int rows;                  // rows of a tile
   int tiles;                 // row tiles of a (observation, key head)
   float* part;               // [slot][rows of a tile][D] unnormalised sums, slot = ((b, h), tile, split)

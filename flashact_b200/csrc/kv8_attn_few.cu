@@ -73,8 +73,9 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
   uint64_t* pfull = sfree + 2;                          // [2] probabilities are in shared memory
   uint64_t* pvdone = pfull + 2;                         // [2] and their product is done
   uint64_t* seen = pvdone + 2;                          // [2] the four warps' maxima are in wmax
-  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(seen + 2);
-  volatile int* err = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  uint64_t* drained = seen + 2;                         // all products are done, after a wait that ran out
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drained + 1);
+  volatile int* err = reinterpret_cast<volatile int*>(tmem_ptr + 1);  // [2] error word, limit of a wait
   uint64_t* maxes = reinterpret_cast<uint64_t*>(state + 480);  // the four warps' maxima are in wmax
   float* rowscale = reinterpret_cast<float*>(state + 512);     // [R]
   int* rowlim = reinterpret_cast<int*>(rowscale + R);          // [R]
@@ -133,7 +134,8 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
       mbar_init(seen + i, 4);
     }
     mbar_init(maxes, 4);
-    *err = 0;
+    mbar_init(drained, 1);
+    err[0] = 0, err[1] = a.spin_limit;
     fence_mbar_init();
     produce<1, C::SLOTS, MT>(ring, full, empty, &kmap, &vmap, t0, nt, (int)hd, err, 0, min(C::SLOTS, 2 * nt));
   }
@@ -192,9 +194,10 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
   const uint32_t tmem_o = tmem + 2 * C::NS;
+  int issued = 0;  // tiles that the producer has sent for
 
   if (w == 0) {
-    if (lane == 0) produce<1, C::SLOTS, MT>(ring, full, empty, &kmap, &vmap, t0, nt, (int)hd, err, min(C::SLOTS, 2 * nt), 2 * nt);
+    if (lane == 0) issued = produce<1, C::SLOTS, MT>(ring, full, empty, &kmap, &vmap, t0, nt, (int)hd, err, min(C::SLOTS, 2 * nt), 2 * nt);
     __syncwarp();
   } else if (w == 1) {
     const int steps = a.dim / 32;
@@ -203,8 +206,8 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
     bool ok = true;
     auto scores = [&](int i) {
       const int pos = pos_k<1>(i), slot = pos % C::SLOTS;
-      ok = ok && mbar_wait(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
-      ok = ok && (i < 2 || mbar_wait(sfree + (i & 1), ((i >> 1) - 1) & 1, err, ERR_SFREE));
+      ok = ok && wait_for(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
+      ok = ok && (i < 2 || wait_for(sfree + (i & 1), ((i >> 1) - 1) & 1, err, ERR_SFREE));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
@@ -212,15 +215,15 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
 #pragma unroll
       for (int k = 0; k < MT * 4; ++k)
         if (k < steps) mma_f8(d, ka + (k >> 2) * 1024 + (k & 3) * 2, qb + (k >> 2) * C::NS * 8 + (k & 3) * 2, ids, k > 0);
-      tc_commit_elect(sfull + (i & 1));
+      if (i > 0 || split != a.fault_split) tc_commit_elect(sfull + (i & 1));
       tc_commit_elect(empty + slot);
     };
     scores(0);
     for (int i = 0; i < nt && ok; ++i) {
       if (i + 1 < nt) scores(i + 1);
       const int pos = pos_v<1>(i, nt), slot = pos % C::SLOTS;
-      ok = ok && mbar_wait(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
-      ok = ok && mbar_wait(pfull + (i & 1), (i >> 1) & 1, err, ERR_P);
+      ok = ok && wait_for(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
+      ok = ok && wait_for(pfull + (i & 1), (i >> 1) & 1, err, ERR_P);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -251,7 +254,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
       const int key = (t0 + i) * TILE + key_lane;
       const float kscale = kn, lv = log2_approx(vn);
       scales(i + 1);
-      ok = mbar_wait(sfull + (i & 1), (i >> 1) & 1, err, ERR_S);
+      ok = wait_for(sfull + (i & 1), (i >> 1) & 1, err, ERR_S);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
         flags[(i & 1) * 4 + quad] = grew;
         mbar_arrive(seen + (i & 1));
       }
-      ok = mbar_wait(seen + (i & 1), (i >> 1) & 1, err, ERR_SEEN);
+      ok = wait_for(seen + (i & 1), (i >> 1) & 1, err, ERR_SEEN);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const int4 fl = *reinterpret_cast<const int4*>(flags + (i & 1) * 4);
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
             *reinterpret_cast<float4*>(wmax + quad * 2 * R + r) = make_float4(x[r], x[r + 1], x[r + 2], x[r + 3]);
           mbar_arrive(maxes);
         }
-        ok = mbar_wait(maxes, grown & 1, err, ERR_SEEN);
+        ok = wait_for(maxes, grown & 1, err, ERR_SEEN);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ++grown;
@@ -325,7 +328,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
           m[r] = mn, d[r] = dn;
         }
         if (i > 0) {
-          ok = mbar_wait(pvdone + ((i - 1) & 1), ((i - 1) >> 1) & 1, err, ERR_PV);
+          ok = wait_for(pvdone + ((i - 1) & 1), ((i - 1) >> 1) & 1, err, ERR_PV);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
@@ -346,7 +349,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
         }
       }
       if (i >= 2) {
-        ok = mbar_wait(pvdone + (i & 1), ((i >> 1) - 1) & 1, err, ERR_PV);
+        ok = wait_for(pvdone + (i & 1), ((i >> 1) - 1) & 1, err, ERR_PV);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
@@ -371,7 +374,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
       if (left < TILE) {
         // keys behind the last limit have P = 0, but their V codes may be NaN: clear them in the tile
         const int pos = pos_v<1>(i, nt), slot = pos % C::SLOTS;
-        ok = mbar_wait(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
+        ok = wait_for(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         clear_behind(ring + slot * C::SLOT, MT * 128, left, st, 128);
@@ -379,7 +382,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
       fence_proxy_async_shared();
       mbar_arrive(pfull + (i & 1));
     }
-    if (ok) ok = mbar_wait(pvdone + ((nt - 1) & 1), ((nt - 1) >> 1) & 1, err, ERR_PV);
+    if (ok) ok = wait_for(pvdone + ((nt - 1) & 1), ((nt - 1) >> 1) & 1, err, ERR_PV);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
     // sums of the rows over the 128 key lanes: through the free P buffers, a warp adds up each fourth row
@@ -413,8 +416,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
           if (r >= nrows) break;
           float x = v[r] + v[R + r] * 0.125f + v[2 * R + r] * (1.0f / 64.0f);
           if (HALF) x += v[(C::PP - 1) * R + r] * (1.0f / 512.0f);
-          x = ok ? x * unit[r] : __int_as_float(0x7fffffff);  // a wait that ran out is seen in the result
-          osum[r * PITCH + d] = x;
+          osum[r * PITCH + d] = x * unit[r];
         }
       }
       __syncwarp();
@@ -422,6 +424,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
     tc_fence_before();
   }
   __syncthreads();
+  if (*err) give_up<C::SLOTS>(full, issued, drained, w == 1, osum, PITCH, PITCH, reinterpret_cast<float*>(mls), 2, R);
   if (w == 1) tmem_dealloc(tmem, C::COLS);
   finish_rows<HALF, MT, 1>(a, osum, PITCH, reinterpret_cast<const float*>(mls), 2, split, b, h, row0, nrows, n, nq, pre, first_part);
 }

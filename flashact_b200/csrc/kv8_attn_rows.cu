@@ -67,8 +67,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* pfull = sfree + 1;                          // probabilities are in tensor memory
   uint64_t* pvdone = pfull + 1;                         // and their product is done
   uint64_t* seen = pvdone + 1;                          // the eight warps' maxima are in half_max
-  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(seen + 1);
-  volatile int* err = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  uint64_t* drained = seen + 1;                         // all products are done, after a wait that ran out
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(drained + 1);
+  volatile int* err = reinterpret_cast<volatile int*>(tmem_ptr + 1);  // [2] error word, limit of a wait
   float* half_max = reinterpret_cast<float*>(state + 512);  // [2][2][128], a tile's maxima in the one of its parity
   signed char* half_exp = reinterpret_cast<signed char*>(state + 2560);  // [2][2][128], the exponent of p vs above each of them
   float* rowscale = half_max + 2 * ROWS;                    // [128], read before the second tile's maxima
@@ -107,7 +108,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     mbar_init(pfull, 256);
     mbar_init(pvdone, 1);
     mbar_init(seen, 8);
-    *err = 0;
+    mbar_init(drained, 2);
+    err[0] = 0, err[1] = a.spin_limit;
     fence_mbar_init();
     produce<2, C::SLOTS, MT>(ring, full, empty, &kmap, &vmap, t0, nt, (int)hd, err, 0, min(C::SLOTS, 2 * nt));
   }
@@ -212,9 +214,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_o = *tmem_ptr, tmem_s = tmem_o + 256, tmem_p = tmem_o + 384;  // O, scores, parts of P (32 columns each)
+  int issued = 0;  // tiles that the producer has sent for
 
   if (w == 0) {
-    if (lane == 0) produce<2, C::SLOTS, MT>(ring, full, empty, &kmap, &vmap, t0, nt, (int)hd, err, min(C::SLOTS, 2 * nt), 2 * nt);
+    if (lane == 0) issued = produce<2, C::SLOTS, MT>(ring, full, empty, &kmap, &vmap, t0, nt, (int)hd, err, min(C::SLOTS, 2 * nt), 2 * nt);
     __syncwarp();
   } else if (w == 1) {
     const int steps = a.dim / 32;
@@ -223,8 +226,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     bool ok = true;
     auto scores = [&](int i) {
       const int pos = pos_k<2>(i), slot = pos % C::SLOTS;
-      ok = ok && mbar_wait(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
-      ok = ok && (i < 1 || mbar_wait(sfree, (i - 1) & 1, err, ERR_SFREE));
+      ok = ok && wait_for(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
+      ok = ok && (i < 1 || wait_for(sfree, (i - 1) & 1, err, ERR_SFREE));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int k = 0; k < MT * 4; ++k)
           if (k < steps) mma_f8(tmem_s, qa + (p * MT + (k >> 2)) * 1024 + (k & 3) * 2, kb + (k >> 2) * 1024 + (k & 3) * 2, ids, p > 0 || k > 0);
-      tc_commit_elect(sfull);
+      if (i > 0 || split != a.fault_split) tc_commit_elect(sfull);
       tc_commit_elect(empty + slot);
     };
     for (int i = 0; i < nt && ok; ++i) scores(i);
@@ -243,8 +246,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     bool ok = true;
     for (int i = 0; i < nt; ++i) {
       const int pos = pos_v<2>(i, nt), slot = pos % C::SLOTS;
-      ok = ok && mbar_wait(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
-      ok = ok && mbar_wait(pfull, i & 1, err, ERR_P);
+      ok = ok && wait_for(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
+      ok = ok && wait_for(pfull, i & 1, err, ERR_P);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -276,7 +279,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // goes through a byte) on their way to the row's other thread. Masked scores are -inf.
     float s[64], f[4], lv[4], mx, mv;
     auto fetch = [&](int i) {
-      ok = mbar_wait(sfull, i & 1, err, ERR_S);
+      ok = wait_for(sfull, i & 1, err, ERR_S);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     fetch(0);
     for (int i = 0; i < nt && ok; ++i) {
-      ok = mbar_wait(seen, i & 1, err, ERR_SEEN);
+      ok = wait_for(seen, i & 1, err, ERR_SEEN);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       {
@@ -334,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         l *= exp2_approx(by);
         m = x, d = dn;
         if (i > 0) {  // O is at rest once the tile before is done
-          ok = mbar_wait(pvdone, (i - 1) & 1, err, ERR_PV);
+          ok = wait_for(pvdone, (i - 1) & 1, err, ERR_PV);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (i + 1 < nt) fetch(i + 1);
       if (!ok) break;
       if (i > 0) {
-        ok = mbar_wait(pvdone, (i - 1) & 1, err, ERR_PV);
+        ok = wait_for(pvdone, (i - 1) & 1, err, ERR_PV);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
@@ -392,7 +395,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int left = top - (t0 + i) * TILE;
       if (left < TILE) {
         const int pos = pos_v<2>(i, nt), slot = pos % C::SLOTS;
-        ok = mbar_wait(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
+        ok = wait_for(full + slot, (pos / C::SLOTS) & 1, err, ERR_FULL);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         clear_behind(ring + slot * C::SLOT, MT * 128, left, st, 256);
@@ -402,15 +405,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_before();
       mbar_arrive(pfull);
     }
-    if (ok) ok = mbar_wait(pvdone, (nt - 1) & 1, err, ERR_PV);
+    if (ok) ok = wait_for(pvdone, (nt - 1) & 1, err, ERR_PV);
     ok = __all_sync(0xffffffffu, ok);
+    if (!ok) tc_wait_st();  // stores that a wait cut off from theirs
     tc_fence_after();
     float* sums = half_max + (nt & 1) * 2 * ROWS;  // the maxima's buffer that the last tile did not use
     sums[half * ROWS + row] = l;
     bar_softmax();
     l = sums[row] + sums[ROWS + row];
     if (half == 0) *reinterpret_cast<float2*>(osum + row * PITCH + MT * 128) = make_float2(m, l);
-    const float norm = ok ? exp2_approx(d - kPTop) : __int_as_float(0x7fffffff);  // a wait that ran out is seen in the result
+    const float norm = exp2_approx(d - kPTop);
 #pragma unroll 1
     for (int c = half * 32; c < a.dim; c += 64) {
       float v[32];
@@ -425,6 +429,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_before();
   }
   __syncthreads();
+  if (*err) give_up<C::SLOTS>(full, issued, drained, w == 1 || w == 2, osum, PITCH, MT * 128, osum + MT * 128, PITCH, ROWS);
   if (w == 1) tmem_dealloc(tmem_o, 512);
   finish_rows<HALF, MT, 4>(a, osum, PITCH, osum + MT * 128, PITCH, split, b, h, row0, nrows, n, nq, pre, first_part);
 }

@@ -298,16 +298,50 @@ __device__ __forceinline__ int pos_v(int i, int n) {
 
 enum { ERR_FULL = 1, ERR_EMPTY, ERR_S, ERR_SFREE, ERR_P, ERR_PV, ERR_SEEN };
 
-// The producer warp's lane: K and V tiles of one head into the ring, in the order of pos_k and pos_v, places from .. to.
+// A bounded wait, as mbar_wait, whose limit stands behind the block's error word (err[1]).
+static __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t phase, volatile int* err, int code) {
+  const uint32_t limit = (uint32_t)err[1];
+  for (uint32_t i = 0; i < limit; ++i) {
+    if (mbar_try_wait(bar, phase)) return true;
+    if ((i & 255u) == 255u) {
+      if (*err) return false;
+      __nanosleep(64);
+    }
+  }
+  atomicCAS((int*)err, 0, code);
+  return false;
+}
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t phase, volatile int* err, int code) {
+  return mbar_test_wait(bar, phase) || wait_slow(bar, phase, err, code);
+}
+
+// The end of a block in which a wait ran out, after all its warps have met: what is in flight ends first (again with a limit), the copies
+// issued and the products, which the issuing warps put on `drained`; then all its rows are NaN, sums and (maximum, sum). A sum that is NaN
+// goes through each join and the merge, where a sum of 0 would be a split without a key. All threads come here.
+template <int SLOTS>
+__device__ __forceinline__ void give_up(uint64_t* full, int issued, uint64_t* drained, bool issuer, float* o, int pitch, int width,
+                                        float* ml, int ml_pitch, int rows) {
+  if (issuer) tc_commit_elect(drained);
+  if (threadIdx.x == 0) {
+    for (int pos = max(0, issued - SLOTS); pos < issued; ++pos)
+      for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(full + pos % SLOTS, (pos / SLOTS) & 1); ++i) {}
+    for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(drained, 0); ++i) {}
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * width; i += blockDim.x) o[i / width * pitch + i % width] = __int_as_float(0x7fffffff);
+  for (int i = threadIdx.x; i < rows; i += blockDim.x) ml[i * ml_pitch] = -INFINITY, ml[i * ml_pitch + 1] = __int_as_float(0x7fffffff);
+  __syncthreads();
+}
+
+// The producer warp's lane: K and V tiles of one head into the ring, in the order of pos_k and pos_v, places from .. to. Returns where it ended.
 template <int LEAD, int SLOTS, int MT>
-__device__ __forceinline__ void produce(unsigned char* ring, uint64_t* full, uint64_t* empty, const CUtensorMap* kmap,
+__device__ __forceinline__ int produce(unsigned char* ring, uint64_t* full, uint64_t* empty, const CUtensorMap* kmap,
                                         const CUtensorMap* vmap, int t0, int nt, int head, volatile int* err, int from,
                                         int to) {
   constexpr int SLOT = MT * 16384;
-  int issued = from;
   for (int pos = from; pos < to; ++pos) {
     const int slot = pos % SLOTS, use = pos / SLOTS;
-    if (use > 0 && !mbar_wait(empty + slot, (use - 1) & 1, err, ERR_EMPTY)) break;
+    if (use > 0 && !wait_for(empty + slot, (use - 1) & 1, err, ERR_EMPTY)) return pos;
     const bool behind = pos >= 2 * nt - min(LEAD, nt), is_v = behind || (pos > LEAD && (pos - LEAD) % 2 != 0);
     const int i = behind ? pos - nt : is_v ? (pos - LEAD - 1) / 2 : pos <= LEAD ? pos : (pos + LEAD) / 2;
     unsigned char* dst = ring + slot * SLOT;
@@ -318,11 +352,8 @@ __device__ __forceinline__ void produce(unsigned char* ring, uint64_t* full, uin
 #pragma unroll
       for (int m = 0; m < MT; ++m) tma_load_3d_plain(dst + m * 16384, kmap, full + slot, m * 128, (t0 + i) * TILE, head);
     }
-    ++issued;
   }
-  if (*err)  // given up: no copy may be in flight when the block ends
-    for (int pos = max(0, issued - SLOTS); pos < issued; ++pos)
-      for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(full + pos % SLOTS, (pos / SLOTS) & 1); ++i) {}
+  return to;
 }
 
 }  // namespace kv8

@@ -197,12 +197,18 @@ FA_API fa_status fa_kv8_read(const fa_kv8* c, const int* lens, int rows, void* k
  * (0: capacity); lengths above it count as it. The work is split by max_len, and the splits are joined in a fixed
  * order: results do not depend on timing. workspace: fa_kv8_attention_workspace bytes, 16-byte aligned,
  * nothing kept in it between calls; calls that overlap on the GPU need one each. Codes behind lens[b]
- * may hold anything; a NaN code before it makes the result of its head NaN, masked or not. */
+ * may hold anything; a NaN code before it makes the result of its head NaN, masked or not. Each wait on the device is bounded; one that
+ * runs out, which no input brings about, is seen in the result, not in the status: the query rows that it served are NaN. */
 FA_API fa_status fa_kv8_attention_workspace(const fa_kv8* c, int tokens, int q_heads, int max_len, size_t* bytes);
 FA_API fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, int q_heads, const fa_rows* q, fa_dtype dtype,
                                   const int* lens, const int* q_lens, const int* prefix, int causal, float scale,
                                   int max_len, const fa_rows* out, void* workspace, size_t workspace_bytes,
                                   fa_stream stream);
+
+/* Test hook, as fa_set_fault_injection, for the fa_kv8_attention calls that follow in this process: the first scores of split
+ * `split` (-1: none) of each tile of rows are never announced, and waits give up after spin_limit polls (0: the default).
+ * No GPU fault. */
+FA_API void fa_kv8_set_fault_injection(int split, unsigned spin_limit);
 
 /* MolmoAct2 action-expert weights (benchmarks/molmoact2/eval_numerics.py:77-100 names), stacked
  * over the L blocks, [out][in] row-major: self_attn.qkv, self_attn.out_proj, cross_attn.q_proj,
