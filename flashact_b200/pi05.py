@@ -33,7 +33,9 @@ def bind_cache(bind, cache, want, valid_len, stream):
     valid_len = [int(x) for x in valid_len]
     if len(valid_len) != cache.batch or min(valid_len) < 0 or max(valid_len) > cache.capacity:
         raise C.FlashActError(C.FA_ERR_INVALID, f"lengths {valid_len} for a cache of {cache.batch} x {cache.capacity} tokens")
-    k, v = cache.read(max(1, max(valid_len)), stream=stream)
+    with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(cache.device)):
+        lens = torch.tensor(valid_len, dtype=torch.int32, device=cache.device)  # what is bound is what is read, whatever cache.lens says
+    k, v = cache.read(max(1, max(valid_len)), lens=lens, stream=stream)
     bind(k, v, valid_len, stream=stream)
 
 
@@ -117,7 +119,8 @@ class Pi05ActionExpert:
     def bind_prefix_cache(self, cache, valid_len=None, stream=None):
         """Binds the prefix held in a Kv8Cache (heads 1, head_dim 256, the engine's layers; K in the split-half RoPE
         order): its values go through bind_prefix_kv as bf16. valid_len (host numbers, as there)
-        defaults to the cache's lengths, which costs a read back."""
+        defaults to the cache's lengths, which costs a read back; given, it may count tokens that are appended and not yet
+        advanced over."""
         bind_cache(self.bind_prefix_kv, cache, (self.cfg.num_layers, 1, 256), valid_len, stream)
 
     def sample_actions(self, noise: torch.Tensor, out: torch.Tensor | None = None, stream=None,
