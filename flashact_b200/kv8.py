@@ -9,7 +9,7 @@ import ctypes
 import torch
 
 from . import _capi as C
-from .pi05 import _DT
+from .pi05 import _DT, on_stream
 
 _byref = ctypes.byref
 _current_device = torch._C._cuda_getDevice
@@ -88,10 +88,6 @@ class Kv8Cache:
         if st != C.FA_OK:
             C.check(self.lib, None, st)
 
-    def _elsewhere(self, stream):
-        """The context in which a call on `stream`, or on a cache of another device than the current one, is made."""
-        return torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.device)
-
     def _rows(self, name, t, heads):
         shape = t.shape
         if len(shape) != 4 or shape[0] != self.batch or shape[2] != heads or shape[3] != self.head_dim:
@@ -116,7 +112,7 @@ class Kv8Cache:
         """Quantises k, v [batch][tokens][heads][head_dim] (fp32, bf16 or fp16, any strides) into `layer` behind `start`
         (default: lens). count (int32 [batch]) gives each observation's number of real rows in a padded batch."""
         if stream is not None or _current_device() != self._index:
-            with self._elsewhere(stream):
+            with on_stream(stream, self._index):
                 return self.append(layer, k, v, count=count, start=start)
         dt = _DT.get(k.dtype)
         if dt is None or v.dtype != k.dtype:
@@ -143,7 +139,7 @@ class Kv8Cache:
         keys up to there, and all below prefix; not causal: every key. max_len: an upper bound of lens that the host knows
         (default: the capacity). Rows of `out` behind q_lens are left as they were (zero in a new tensor)."""
         if stream is not None or _current_device() != self._index:
-            with self._elsewhere(stream):
+            with on_stream(stream, self._index):
                 return self.attend(layer, q, scale=scale, causal=causal, prefix=prefix, q_lens=q_lens, lens=lens,
                                    max_len=max_len, out=out)
         dt, shape = _DT.get(q.dtype), q.shape
@@ -174,7 +170,7 @@ class Kv8Cache:
     def read(self, rows: int, *, dtype=torch.bfloat16, lens: torch.Tensor | None = None, stream=None):
         """(K, V) as values [batch][layers][rows][heads * head_dim], zero at and behind each length."""
         if stream is not None or _current_device() != self._index:
-            with self._elsewhere(stream):
+            with on_stream(stream, self._index):
                 return self.read(rows, dtype=dtype, lens=lens)
         if dtype not in _DT:
             raise _bad(f"values are fp32, bf16 or fp16, not {dtype}")

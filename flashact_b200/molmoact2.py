@@ -76,7 +76,7 @@ class MolmoAct2ActionExpert:
         """Binds the cross-attention context held in a Kv8Cache (heads 8, head_dim 96, the engine's layers): its
         values go through bind_context as bf16. ctx_len defaults to the cache's lengths, which costs a read back; given, it may count
         tokens that are appended and not yet advanced over."""
-        bind_cache(self.bind_context, cache, (self.cfg.num_layers, 8, 96), ctx_len, stream)
+        bind_cache(self, self.bind_context, cache, (self.cfg.num_layers, 8, 96), ctx_len, stream)
 
     def sample_actions(self, noise: torch.Tensor, out=None, stream=None, sync=True):
         noise = noise.float().contiguous()

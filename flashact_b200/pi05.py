@@ -22,21 +22,32 @@ def _stream_ptr(stream=None):
     return ctypes.c_void_p(s.cuda_stream)
 
 
-def bind_cache(bind, cache, want, valid_len, stream):
-    """Reads a Kv8Cache of `want` = (layers, heads, head_dim) and hands its values to an engine's bind."""
+def on_stream(stream, device: int):
+    """The context of a call on `stream`, or (None) on the current stream of `device`, whose memory it works on."""
+    if stream is None:
+        return torch.cuda.device(device)
+    if stream.device_index != device:
+        raise C.FlashActError(C.FA_ERR_INVALID, f"a stream of cuda:{stream.device_index} for memory on cuda:{device}")
+    return torch.cuda.stream(stream)
+
+
+def bind_cache(engine, bind, cache, want, valid_len, stream):
+    """Reads a Kv8Cache of `want` = (layers, heads, head_dim) and hands its values to an engine's bind, all on one stream of the
+    engine's device."""
+    if cache.device.index != engine.device:
+        raise C.FlashActError(C.FA_ERR_INVALID, f"a cache on {cache.device}: the engine is on cuda:{engine.device}")
     have = (cache.layers, cache.heads, cache.head_dim)
     if have != want:
         raise C.FlashActError(C.FA_ERR_INVALID, f"a cache of layers, heads, head_dim {have}: the engine has {want}")
-    if valid_len is None:
-        with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(cache.device)):
+    with on_stream(stream, engine.device):
+        if valid_len is None:
             valid_len = cache.lens.tolist()
-    valid_len = [int(x) for x in valid_len]
-    if len(valid_len) != cache.batch or min(valid_len) < 0 or max(valid_len) > cache.capacity:
-        raise C.FlashActError(C.FA_ERR_INVALID, f"lengths {valid_len} for a cache of {cache.batch} x {cache.capacity} tokens")
-    with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(cache.device)):
+        valid_len = [int(x) for x in valid_len]
+        if len(valid_len) != cache.batch or min(valid_len) < 0 or max(valid_len) > cache.capacity:
+            raise C.FlashActError(C.FA_ERR_INVALID, f"lengths {valid_len} for a cache of {cache.batch} x {cache.capacity} tokens")
         lens = torch.tensor(valid_len, dtype=torch.int32, device=cache.device)  # what is bound is what is read, whatever cache.lens says
-    k, v = cache.read(max(1, max(valid_len)), lens=lens, stream=stream)
-    bind(k, v, valid_len, stream=stream)
+        k, v = cache.read(max(1, max(valid_len)), lens=lens)
+        bind(k, v, valid_len)
 
 
 class Pi05ActionExpert:
@@ -121,7 +132,7 @@ class Pi05ActionExpert:
         order): its values go through bind_prefix_kv as bf16. valid_len (host numbers, as there)
         defaults to the cache's lengths, which costs a read back; given, it may count tokens that are appended and not yet
         advanced over."""
-        bind_cache(self.bind_prefix_kv, cache, (self.cfg.num_layers, 1, 256), valid_len, stream)
+        bind_cache(self, self.bind_prefix_kv, cache, (self.cfg.num_layers, 1, 256), valid_len, stream)
 
     def sample_actions(self, noise: torch.Tensor, out: torch.Tensor | None = None, stream=None,
                        sync: bool = True) -> torch.Tensor:

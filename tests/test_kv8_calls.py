@@ -1,4 +1,6 @@
 """Calls of the 8-bit KV cache and the NVFP4 linear layer at the edges of what their documentation allows."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -27,4 +29,58 @@ def test_bind_of_tokens_that_lens_does_not_count_yet(require_gpu):
         cache.lens.copy_(_dev(lens))
         eng.bind_prefix_cache(cache, [120, 90])
         assert torch.equal(eng.sample_actions(c.noise.cuda()), want), lens
+    eng.close()
+
+
+def test_bind_refuses_another_device():
+    """Values are read, copied and bound on one stream of one device."""
+    from flashact_b200 import FlashActError
+    from flashact_b200.pi05 import bind_cache
+    cache = SimpleNamespace(device=torch.device("cuda", 0), layers=2, heads=1, head_dim=256, batch=1, capacity=64)
+    with pytest.raises(FlashActError, match="the engine is on cuda:1"):
+        bind_cache(SimpleNamespace(device=1), None, cache, (2, 1, 256), [3], None)
+    with pytest.raises(FlashActError, match="a stream of cuda:1"):
+        bind_cache(SimpleNamespace(device=0), None, cache, (2, 1, 256), [3], SimpleNamespace(device_index=1))
+
+
+@pytest.mark.gpu
+def test_streams_of_another_device_are_refused(require_gpu):
+    """They would not be the stream that the call then runs on."""
+    from flashact_b200 import FlashActError, Kv8Cache
+    from flashact_b200.quant import nvfp4_linear
+    other = SimpleNamespace(device_index=1)
+    c = Kv8Cache(1, 1, 1, 64, 64)
+    k = torch.zeros(1, 1, 1, 64, dtype=BF, device="cuda")
+    x, w, bs, ts = (torch.zeros(*n, dtype=t, device="cuda") for n, t in (((1, 64), BF), ((8, 32), torch.uint8), ((8, 4), torch.uint8),
+                                                                        ((1,), torch.float32)))
+    for f in (lambda: c.append(0, k, k, stream=other), lambda: c.attend(0, k, stream=other), lambda: c.read(1, stream=other),
+              lambda: nvfp4_linear(x, w, bs, ts, stream=other)):
+        with pytest.raises(FlashActError, match="a stream of cuda:1"):
+            f()
+
+
+@pytest.mark.gpu
+def test_bind_on_a_side_stream(require_gpu):
+    """Read and bound on the stream that is given, or on the current one where that is not the default."""
+    from flashact_b200 import Kv8Cache
+    from oracle import pi05_oracle as O
+    from tests.pi05_util import engine_for
+    c = O.make_case(seed=7, L=2, T=50, AD=32, Lp=64, B=1, num_steps=2)
+    eng = engine_for(c)
+    side = torch.cuda.Stream()
+    got = []
+    for how in (0, 1, 2):
+        cache = Kv8Cache(1, 2, 1, 256, 64)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side if how else torch.cuda.current_stream()):
+            for layer in range(2):
+                cache.append(layer, c.k[:, layer, :, None].contiguous().cuda(), c.v[:, layer, :, None].contiguous().cuda())
+            cache.advance(64)
+            if how < 2:
+                eng.bind_prefix_cache(cache)
+        if how == 2:
+            eng.bind_prefix_cache(cache, stream=side)
+        torch.cuda.synchronize()
+        got.append(eng.sample_actions(c.noise.cuda()))
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
     eng.close()
