@@ -126,9 +126,11 @@ class Kv8Cache:
                                  self._lens if start is None else self._ints("start", start), self._ints("count", count),
                                  _current_stream(self._index)))
 
-    def advance(self, n):
-        """lens += n (a number, or a tensor [batch]) after every layer has appended."""
-        self.lens += n
+    def advance(self, n, *, stream=None):
+        """lens += n (a number, or a tensor [batch]) after every layer has appended, on the stream of the appends: those on `stream` that
+        have not run yet still read the lengths."""
+        with on_stream(stream, self._index):
+            self._lens_tensor += n
 
     def attend(self, layer: int, q: torch.Tensor, *, scale: float | None = None, causal: bool = True,
                prefix: torch.Tensor | None = None, q_lens: torch.Tensor | None = None, lens: torch.Tensor | None = None,

@@ -84,3 +84,26 @@ def test_bind_on_a_side_stream(require_gpu):
         got.append(eng.sample_actions(c.noise.cuda()))
     assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
     eng.close()
+
+
+@pytest.mark.gpu
+def test_advance_on_the_stream_of_the_appends(require_gpu):
+    """A step on a side stream that is behind the current one: every layer appends at the same place, then the lengths move."""
+    from flashact_b200 import Kv8Cache
+    k = torch.randn(1, 5, 1, 64, generator=torch.Generator().manual_seed(0)).to(BF).cuda()
+    here, there = Kv8Cache(1, 3, 1, 64, 64), Kv8Cache(1, 3, 1, 64, 64)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # some ms
+    for c, s in ((here, None), (there, side)):
+        for _ in range(2):
+            for layer in range(3):
+                c.append(layer, k, k, stream=s)
+            c.advance(5, stream=s)
+    torch.cuda.synchronize()
+    assert here.lens.tolist() == there.lens.tolist() == [10]
+    assert torch.equal(here.k, there.k) and torch.equal(here.v, there.v) and torch.equal(here.k_scale, there.k_scale)
+    with pytest.raises(RuntimeError):
+        here.advance(torch.ones(2, dtype=torch.int32, device="cuda"))
+    assert here.lens.tolist() == [10]
