@@ -84,6 +84,9 @@ class Kv8Cache:
     def lens(self, t):
         self._lens, self._lens_tensor = self._ints("lens", t), t
 
+    def tensors(self):
+        return self.k, self.v, self.k_scale, self.v_scale, self._lens_tensor
+
     def _check(self, st):
         if st != C.FA_OK:
             C.check(self.lib, None, st)
@@ -112,7 +115,7 @@ class Kv8Cache:
         """Quantises k, v [batch][tokens][heads][head_dim] (fp32, bf16 or fp16, any strides) into `layer` behind `start`
         (default: lens). count (int32 [batch]) gives each observation's number of real rows in a padded batch."""
         if stream is not None or _current_device() != self._index:
-            with on_stream(stream, self._index):
+            with on_stream(stream, self._index, k, v, count, start, *self.tensors()):
                 return self.append(layer, k, v, count=count, start=start)
         dt = _DT.get(k.dtype)
         if dt is None or v.dtype != k.dtype:
@@ -129,7 +132,7 @@ class Kv8Cache:
     def advance(self, n, *, stream=None):
         """lens += n (a number, or a tensor [batch]) after every layer has appended, on the stream of the appends: those on `stream` that
         have not run yet still read the lengths."""
-        with on_stream(stream, self._index):
+        with on_stream(stream, self._index, self._lens_tensor, n if isinstance(n, torch.Tensor) else None):
             self._lens_tensor += n
 
     def attend(self, layer: int, q: torch.Tensor, *, scale: float | None = None, causal: bool = True,
@@ -141,7 +144,7 @@ class Kv8Cache:
         keys up to there, and all below prefix; not causal: every key. max_len: an upper bound of lens that the host knows
         (default: the capacity). Rows of `out` behind q_lens are left as they were (zero in a new tensor)."""
         if stream is not None or _current_device() != self._index:
-            with on_stream(stream, self._index):
+            with on_stream(stream, self._index, q, prefix, q_lens, lens, out, *self.tensors()):
                 return self.attend(layer, q, scale=scale, causal=causal, prefix=prefix, q_lens=q_lens, lens=lens,
                                    max_len=max_len, out=out)
         dt, shape = _DT.get(q.dtype), q.shape
@@ -172,7 +175,7 @@ class Kv8Cache:
     def read(self, rows: int, *, dtype=torch.bfloat16, lens: torch.Tensor | None = None, stream=None):
         """(K, V) as values [batch][layers][rows][heads * head_dim], zero at and behind each length."""
         if stream is not None or _current_device() != self._index:
-            with on_stream(stream, self._index):
+            with on_stream(stream, self._index, lens, *self.tensors()):
                 return self.read(rows, dtype=dtype, lens=lens)
         if dtype not in _DT:
             raise _bad(f"values are fp32, bf16 or fp16, not {dtype}")

@@ -22,12 +22,16 @@ def _stream_ptr(stream=None):
     return ctypes.c_void_p(s.cuda_stream)
 
 
-def on_stream(stream, device: int):
-    """The context of a call on `stream`, or (None) on the current stream of `device`, whose memory it works on."""
+def on_stream(stream, device: int, *tensors):
+    """The context of a call on `stream`, or (None) on the current stream of `device`, whose memory it works on. `tensors` (or None) are
+    what the call uses: their memory is not given to anyone else before `stream` is done with it, whenever the caller drops them."""
     if stream is None:
         return torch.cuda.device(device)
     if stream.device_index != device:
         raise C.FlashActError(C.FA_ERR_INVALID, f"a stream of cuda:{stream.device_index} for memory on cuda:{device}")
+    for t in tensors:
+        if t is not None and t.is_cuda:
+            t.record_stream(stream)
     return torch.cuda.stream(stream)
 
 
@@ -39,7 +43,7 @@ def bind_cache(engine, bind, cache, want, valid_len, stream):
     have = (cache.layers, cache.heads, cache.head_dim)
     if have != want:
         raise C.FlashActError(C.FA_ERR_INVALID, f"a cache of layers, heads, head_dim {have}: the engine has {want}")
-    with on_stream(stream, engine.device):
+    with on_stream(stream, engine.device, *cache.tensors()):
         if valid_len is None:
             valid_len = cache.lens.tolist()
         valid_len = [int(x) for x in valid_len]

@@ -67,7 +67,7 @@ def nvfp4_linear(x: torch.Tensor, packed: torch.Tensor, block_scale: torch.Tenso
     if dt is None or not shape or index < 0:
         raise C.FlashActError(C.FA_ERR_INVALID, "x must be a CUDA tensor [..., K]")
     if stream is not None or torch._C._cuda_getDevice() != index:
-        with on_stream(stream, index):
+        with on_stream(stream, index, x, packed, block_scale, tensor_scale, bias, out):
             return nvfp4_linear(x, packed, block_scale, tensor_scale, bias=bias, out=out)
     K, pshape = shape[-1], packed.shape
     N = pshape[0] if len(pshape) == 2 else 0

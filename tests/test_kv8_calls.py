@@ -36,7 +36,7 @@ def test_bind_refuses_another_device():
     """Values are read, copied and bound on one stream of one device."""
     from flashact_b200 import FlashActError
     from flashact_b200.pi05 import bind_cache
-    cache = SimpleNamespace(device=torch.device("cuda", 0), layers=2, heads=1, head_dim=256, batch=1, capacity=64)
+    cache = SimpleNamespace(device=torch.device("cuda", 0), layers=2, heads=1, head_dim=256, batch=1, capacity=64, tensors=lambda: ())
     with pytest.raises(FlashActError, match="the engine is on cuda:1"):
         bind_cache(SimpleNamespace(device=1), None, cache, (2, 1, 256), [3], None)
     with pytest.raises(FlashActError, match="a stream of cuda:1"):
@@ -107,3 +107,40 @@ def test_advance_on_the_stream_of_the_appends(require_gpu):
     with pytest.raises(RuntimeError):
         here.advance(torch.ones(2, dtype=torch.int32, device="cuda"))
     assert here.lens.tolist() == [10]
+
+
+@pytest.mark.gpu
+def test_inputs_dropped_before_a_side_stream_has_run(require_gpu):
+    """Temporaries handed to a call on another stream keep their memory until that stream is done with them."""
+    from flashact_b200 import Kv8Cache
+    from flashact_b200.quant import nvfp4_linear
+    g = torch.Generator().manual_seed(2)
+    k = torch.randn(2, 300, 2, 64, generator=g).to(BF).cuda()
+    q = torch.randn(2, 40, 4, 64, generator=g).to(BF).cuda()
+    x = torch.randn(16, 4096, generator=g).to(BF).cuda()
+    w = [torch.randint(0, 256, (640, 2048), generator=g, dtype=torch.uint8).cuda(),
+         torch.randint(0, 100, (640, 256), generator=g, dtype=torch.uint8).cuda(), torch.tensor([1e-4], device="cuda")]
+    n = _dev([300, 200])
+    want = Kv8Cache(2, 1, 2, 64, 512)
+    want.append(0, k, k, count=n)
+    want.advance(n)
+    attended, linear = want.attend(0, q), nvfp4_linear(x, *w)
+    side = torch.cuda.Stream()
+    got = Kv8Cache(2, 1, 2, 64, 512)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(40_000_000)  # longer than the host needs for what follows
+    # the clones are made on the current stream, which is idle: their values are there long before the side stream gets to them
+    tmp = [t.clone() for t in (k, k, n, q, x, n)]
+    torch.cuda.current_stream().synchronize()
+    got.append(0, tmp[0], tmp[1], count=tmp[2], stream=side)
+    got.advance(tmp[5], stream=side)
+    a = got.attend(0, tmp[3], stream=side)
+    y = nvfp4_linear(tmp[4], *w, stream=side)
+    sizes = [(t.shape, t.dtype) for t in tmp]
+    del tmp
+    for shape, dt in sizes * 4:  # whoever asks next
+        torch.full(shape, 1, dtype=dt, device="cuda")
+    torch.cuda.synchronize()
+    assert torch.equal(got.k, want.k) and torch.equal(got.v, want.v) and torch.equal(got.lens, want.lens)
+    assert torch.equal(a, attended) and torch.equal(y, linear)
