@@ -196,7 +196,9 @@ FA_API fa_status fa_kv8_read(const fa_kv8* c, const int* lens, int rows, void* k
  * causal: all lens[b]. A query that sees no key gets zeros. max_len is an upper bound of lens known to the host
  * (0: capacity); lengths above it count as it. The work is split by max_len, and the splits are joined in a fixed
  * order: results do not depend on timing. workspace: fa_kv8_attention_workspace bytes, 16-byte aligned,
- * nothing kept in it between calls; calls that overlap on the GPU need one each. Codes behind lens[b]
+ * nothing kept in it between calls; calls that overlap on the GPU need one each. The need follows the splits and does not grow with the
+ * sizes: one token over a long cache may need more than a prompt, which needs none. One workspace for several calls is the
+ * largest of what each of their (cache, tokens, q_heads, max_len) asks for. Codes behind lens[b]
  * may hold anything; a NaN code before it makes the result of its head NaN, masked or not. Each wait on the device is bounded; one that
  * runs out, which no input brings about, is seen in the result, not in the status: the query rows that it served are NaN. */
 FA_API fa_status fa_kv8_attention_workspace(const fa_kv8* c, int tokens, int q_heads, int max_len, size_t* bytes);

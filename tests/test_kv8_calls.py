@@ -1,4 +1,5 @@
 """Calls of the 8-bit KV cache and the NVFP4 linear layer at the edges of what their documentation allows."""
+import ctypes
 from types import SimpleNamespace
 
 import pytest
@@ -144,3 +145,30 @@ def test_inputs_dropped_before_a_side_stream_has_run(require_gpu):
     torch.cuda.synchronize()
     assert torch.equal(got.k, want.k) and torch.equal(got.v, want.v) and torch.equal(got.lens, want.lens)
     assert torch.equal(a, attended) and torch.equal(y, linear)
+
+
+def test_one_workspace_for_several_calls():
+    """The workspace of a large call need not do for a smaller one; the largest of what the calls ask for does for each of them."""
+    from flashact_b200 import _capi as C
+    from flashact_b200.build import build
+    lib = C.load_library(build())
+    c = C.FaKv8(16, 16, 16, 16, 1, 1, 1, 256, 1 << 14, 64)
+    r = C.FaRows(16, 256, 256, 256)
+
+    def need(tokens, max_len):
+        n = ctypes.c_size_t()
+        assert lib.fa_kv8_attention_workspace(ctypes.byref(c), tokens, 8, max_len, ctypes.byref(n)) == C.FA_OK
+        return n.value
+
+    def attend(tokens, max_len, ws):
+        st = lib.fa_kv8_attention(ctypes.byref(c), 0, tokens, 8, ctypes.byref(r), C.FA_DT_BF16, 16, None, None, 1, 0.1, max_len,
+                                  ctypes.byref(r), 16, ws, None)
+        return st, lib.fa_last_error(None).decode()
+    calls = [(t, n) for t in (1, 2, 16, 50, 256, 1024) for n in (0, 128, 1024, 9000)]
+    needs = [need(*x) for x in calls]
+    assert need(1024, 0) < need(1, 0)
+    st, why = attend(1, 0, need(1024, 0))
+    assert st == C.FA_ERR_INVALID and "workspace" in why
+    for x in calls:
+        st, why = attend(*x, max(needs))
+        assert "workspace of" not in why  # whatever else these made-up pointers are refused for
