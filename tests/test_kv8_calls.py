@@ -172,3 +172,45 @@ def test_one_workspace_for_several_calls():
     for x in calls:
         st, why = attend(*x, max(needs))
         assert "workspace of" not in why  # whatever else these made-up pointers are refused for
+
+
+@pytest.mark.gpu
+def test_values_past_32_bits(require_gpu):
+    """More than 2^32 codes in K and in V: what append wrote at the end of each head, found there by torch's own indexing, is the reference's; read
+    gives it back, and attention weighs it against a million keys of zero."""
+    from flashact_b200 import Kv8Cache
+    from tests.kv8_util import codes, scale_of, values
+    B, heads, D, cap = 3, 6, 256, 1 << 20
+    c = Kv8Cache(B, 1, heads, D, cap, block=128)
+    assert c.k.numel() > 1 << 32
+    n = cap - 3
+    g = torch.Generator().manual_seed(9)
+    k, v = torch.randn(B, 2, heads, D, generator=g).to(BF), (torch.randn(B, 2, heads, D, generator=g) * 1000).to(BF)
+    q = torch.randn(B, 1, heads, D, generator=g)
+    q = (q + 1.3 * k.float().mean(1, keepdim=True)).to(BF)  # scores near log(cap), so that both sides count
+    c.lens.fill_(n - 2)
+    c.append(0, k.cuda(), v.cuda())
+    c.advance(2)
+    got = c.attend(0, q.cuda()).cpu().double()
+    kk, vv = c.read(cap)
+    assert (kk[:, 0, n - 130:n - 2] == 0).all() and (vv[:, 0, n:] == 0).all()
+    for b in range(B):
+        for h in range(heads):
+            real = []
+            for name, new, x in (("k", k, kk), ("v", v, vv)):
+                x32 = new[b, :, h].float()
+                s = scale_of(x32.abs().max().item())
+                want = codes(x32, s)
+                held = (c.k[b, 0, h, n - 2:n] if name == "k" else c.v[b, 0, h, :, n - 2:n].t()).cpu()
+                assert torch.equal(held, want) and (c.k_scale if name == "k" else c.v_scale)[b, 0, h, -1].item() == s
+                real.append(values(want) * s)
+                assert torch.equal(x[b, 0, n - 2:n, h * D:(h + 1) * D].cpu().double(), real[-1])
+            a = real[0] @ q[b, 0, h].double() / D ** 0.5
+            p = torch.exp(a)
+            p = p / (p.sum() + n - 2)
+            o, spread = p @ real[1], p @ real[1].abs()
+            big = (real[0].abs() @ q[b, 0, h].double().abs()).max().item() / D ** 0.5
+            # roundings as in tests/kv8_bounds.py: output, products of P, scores and exponentials; the sum of a million ones in fp32, at most
+            # 2^20 / 128 of them to a thread, is exact
+            tol = 2.0 ** -8 * o.abs() + 1.01 * (2.0 ** -11 + 2 * ((D + 8) * 2.0 ** -23 * big + 2.0 ** -17 + 2.0 ** -20)) * spread
+            assert p.min() > 1e-9 and ((got[b, 0, h] - o).abs() <= tol).all(), (b, h, p.tolist(), ((got[b, 0, h] - o).abs() / tol).max().item())
