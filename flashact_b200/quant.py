@@ -62,7 +62,7 @@ def nvfp4_linear(x: torch.Tensor, packed: torch.Tensor, block_scale: torch.Tenso
                  bias: torch.Tensor | None = None, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """x W^T * tensor_scale (+ bias) for x [..., K] (bf16 or fp16) of up to 16 rows and one layer's matrix as
     quantize_nvfp4 gives it: packed uint8 [N, K/2], block_scale uint8 [N, K/16], tensor_scale fp32 of one element;
-    bias fp32 [N]. Returns [..., N] in x's type."""
+    bias fp32 [N]. Returns [..., N] in x's type; `out` may not overlap x."""
     dt, shape, index = _DT.get(x.dtype), x.shape, x.get_device()
     if dt is None or not shape or index < 0:
         raise C.FlashActError(C.FA_ERR_INVALID, "x must be a CUDA tensor [..., K]")

@@ -138,7 +138,7 @@ FA_API fa_status fa_quantize_nvfp4(const void* w, fa_dtype dtype, int L, int row
  * (packed [N][K/2], block_scale [N][K/16], tensor_scale one fp32): the codes are read as they are, 9/16 of a
  * byte a weight, and their products with the block scales are exact in x's type. x [M][K] (row stride ldx,
  * a multiple of 8) and y [M][N] (row stride ldy) in `dtype` (bf16 or fp16), bias fp32 [N] or NULL; M <= 16
- * (0: nothing is done), K a multiple of 16. Sums are fp32, rounded once. Device memory of the current
+ * (0: nothing is done), K a multiple of 16; no element of y is one of x. Sums are fp32, rounded once. Device memory of the current
  * device, x 16-byte and packed 8-byte aligned; asynchronous on `stream`, no workspace, results do not
  * depend on timing. Errors are read with fa_last_error(NULL). */
 FA_API fa_status fa_nvfp4_linear(const void* x, fa_dtype dtype, int M, int K, long long ldx, const unsigned char* packed,

@@ -214,3 +214,19 @@ def test_values_past_32_bits(require_gpu):
             # 2^20 / 128 of them to a thread, is exact
             tol = 2.0 ** -8 * o.abs() + 1.01 * (2.0 ** -11 + 2 * ((D + 8) * 2.0 ** -23 * big + 2.0 ** -17 + 2.0 ** -20)) * spread
             assert p.min() > 1e-9 and ((got[b, 0, h] - o).abs() <= tol).all(), (b, h, p.tolist(), ((got[b, 0, h] - o).abs() / tol).max().item())
+
+
+def test_linear_refuses_an_output_over_its_input():
+    """Blocks write y while others read x. Rows beside each other in one buffer do not overlap."""
+    from flashact_b200 import _capi as C
+    from flashact_b200.build import build
+    lib = C.load_library(build())
+
+    def call(x, y, M, K, ldx, N, ldy):
+        st = lib.fa_nvfp4_linear(x, C.FA_DT_BF16, M, K, ldx, 1 << 20, 1 << 20, 1 << 20, None, N, y, ldy, None)
+        return st == C.FA_ERR_INVALID and "overlaps" in lib.fa_last_error(None).decode()
+    assert call(4096, 4096, 1, 64, 64, 64, 64) and call(4096, 4096, 16, 64, 64, 64, 64)
+    assert call(4096, 4096 + 2 * 63, 1, 64, 64, 8, 8) and not call(4096, 4096 + 2 * 64, 1, 64, 64, 8, 8)
+    assert call(4096, 4096 - 2 * 7, 1, 64, 64, 8, 8) and not call(4096, 4096 - 2 * 8, 1, 64, 64, 8, 8)
+    # columns 0..63 are x, 64..95 are y, of rows of 96
+    assert not call(4096, 4096 + 2 * 64, 16, 64, 96, 32, 96) and call(4096, 4096 + 2 * 64, 16, 64, 96, 33, 96)
