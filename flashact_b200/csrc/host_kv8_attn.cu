@@ -153,6 +153,8 @@ extern "C" fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, in
   if (prefix && !causal) return fail(nullptr, FA_ERR_INVALID, "a prefix belongs to a causal mask");
   if (reinterpret_cast<uintptr_t>(q->ptr) % 2 || reinterpret_cast<uintptr_t>(out->ptr) % 2)
     return fail(nullptr, FA_ERR_INVALID, "queries and output must be aligned to their type");
+  if ((c->batch > 1 && !out->batch) || (tokens > 1 && !out->token) || (q_heads > 1 && !out->head))
+    return fail(nullptr, FA_ERR_INVALID, "rows of the output lie on one another (a stride of 0)");
   if (tokens == 0) return FA_OK;
   const int top = max_len ? max_len : c->capacity;
   int device = 0;

@@ -142,7 +142,8 @@ class Kv8Cache:
         defaults to head_dim ** -0.5. lens (default: the cache's) counts the cached tokens, the queries' own among
         them. causal: token i of an observation's q_lens (default: tokens) stands at lens - q_lens + i and sees the
         keys up to there, and all below prefix; not causal: every key. max_len: an upper bound of lens that the host knows
-        (default: the capacity). Rows of `out` behind q_lens are left as they were (zero in a new tensor)."""
+        (default: the capacity). `out` may be q itself, but may not overlap it in another way. Its rows behind
+        q_lens are left as they were (zero in a new tensor)."""
         if stream is not None or _current_device() != self._index:
             with on_stream(stream, self._index, q, prefix, q_lens, lens, out, *self.tensors()):
                 return self.attend(layer, q, scale=scale, causal=causal, prefix=prefix, q_lens=q_lens, lens=lens,

@@ -188,7 +188,8 @@ FA_API fa_status fa_kv8_read(const fa_kv8* c, const int* lens, int rows, void* k
 /* Attention of `tokens` query tokens over layer `layer`: out = softmax(scale q K^T + mask) V, rounded once to the queries' type
  * (`dtype`: bf16 or f16). Scores, maxima and sums are fp32; what goes into the products has fewer bits than that: a probability
  * times its V scale is off by at most 2^-11 of itself (f16 queries 2^-15) and by 2^-29 of the largest such product that the row sees,
- * and an element of a query by 2^-17 of the row's largest element (2^-21 with up to 16 query rows of a key head). q and out are [batch][tokens][q_heads][head_dim] rows; query head
+ * and an element of a query by 2^-17 of the row's largest element (2^-21 with up to 16 query rows of a key head). q and out are [batch][tokens][q_heads][head_dim] rows; out may be q
+ * (the same pointer and strides), but for that its rows overlap neither q nor one another; query head
  * i reads key head i / (q_heads / heads). lens, q_lens, prefix: device int32 [batch]. lens[b] tokens
  * of observation b are in the cache, the queries' own included where they attend to themselves; q_lens[b] (NULL:
  * tokens) of its query tokens are real: the output rows of the others are left as they were. Query token i

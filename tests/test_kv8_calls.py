@@ -230,3 +230,20 @@ def test_linear_refuses_an_output_over_its_input():
     assert call(4096, 4096 - 2 * 7, 1, 64, 64, 8, 8) and not call(4096, 4096 - 2 * 8, 1, 64, 64, 8, 8)
     # columns 0..63 are x, 64..95 are y, of rows of 96
     assert not call(4096, 4096 + 2 * 64, 16, 64, 96, 32, 96) and call(4096, 4096 + 2 * 64, 16, 64, 96, 33, 96)
+
+
+def test_attention_refuses_output_rows_on_one_another():
+    """An expanded output: all rows of it would be written to one place, in no order."""
+    from flashact_b200 import _capi as C
+    from flashact_b200.build import build
+    lib = C.load_library(build())
+    c = C.FaKv8(16, 16, 16, 16, 2, 1, 1, 64, 128, 64)
+    q = C.FaRows(16, 512, 128, 64)
+
+    def refused(tokens, heads, batch, token, head):
+        o = C.FaRows(16, batch, token, head)
+        st = lib.fa_kv8_attention(ctypes.byref(c), 0, tokens, heads, ctypes.byref(q), C.FA_DT_BF16, 16, None, None, 1, 0.1, 0,
+                                  ctypes.byref(o), None, 0, None)
+        return st == C.FA_ERR_INVALID and "stride of 0" in lib.fa_last_error(None).decode()
+    assert refused(4, 2, 0, 128, 64) and refused(4, 2, 512, 0, 64) and refused(4, 2, 512, 128, 0)
+    assert not refused(4, 2, 512, 128, 64) and not refused(1, 1, 64, 0, 0)
