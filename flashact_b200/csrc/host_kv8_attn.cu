@@ -149,7 +149,8 @@ extern "C" fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, in
   if (dtype != FA_DT_BF16 && dtype != FA_DT_F16)
     return fail(nullptr, FA_ERR_UNSUPPORTED, "queries are bf16 or fp16 (dtype %d)", (int)dtype);
   if (!q || !out) return fail(nullptr, FA_ERR_INVALID, "null queries or output");
-  if (!(std::fabs(scale) <= 3.0e38f)) return fail(nullptr, FA_ERR_INVALID, "the scale is not a finite number");
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!std::isfinite(scale_log2)) return fail(nullptr, FA_ERR_INVALID, "the scale is not a finite number, or its product with log2 e is none");
   if (prefix && !causal) return fail(nullptr, FA_ERR_INVALID, "a prefix belongs to a causal mask");
   if (reinterpret_cast<uintptr_t>(q->ptr) % 2 || reinterpret_cast<uintptr_t>(out->ptr) % 2)
     return fail(nullptr, FA_ERR_INVALID, "queries and output must be aligned to their type");
@@ -182,7 +183,7 @@ extern "C" fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, in
   a.blocks = c->capacity / c->block, a.block_log2 = __builtin_ctz(c->block), a.half = dtype == FA_DT_F16;
   a.q_wide = reinterpret_cast<uintptr_t>(q->ptr) % 16 == 0 && q->batch % 8 == 0 && q->token % 8 == 0 && q->head % 8 == 0;
   a.o_wide = reinterpret_cast<uintptr_t>(out->ptr) % 8 == 0 && out->batch % 4 == 0 && out->token % 4 == 0 && out->head % 4 == 0;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale_log2;
   a.group_mul = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
   a.nsplit = p.nsplit, a.cluster = p.cluster, a.split_chunks = p.split_chunks, a.rows = p.rows, a.tiles = p.tiles;
   a.part = reinterpret_cast<float*>(workspace);

@@ -47,7 +47,9 @@ class Kv8Cache:
         [head_dim], v uint8 [batch][layers][heads][head_dim][capacity], scales fp32 [batch][layers][heads][blocks],
         lens int32 [batch]; contiguous, on one GPU."""
         self = cls.__new__(cls)
-        self._own(k, v, k_scale, v_scale, torch.zeros(k.shape[0], dtype=torch.int32, device=k.device) if lens is None else lens)
+        if lens is None and k.dim():
+            lens = torch.zeros(k.shape[0], dtype=torch.int32, device=k.device)
+        self._own(k, v, k_scale, v_scale, lens)
         return self
 
     def _own(self, k, v, k_scale, v_scale, lens):
@@ -82,6 +84,8 @@ class Kv8Cache:
 
     @lens.setter
     def lens(self, t):
+        if t is None:
+            raise _bad("'lens' must be a tensor")
         self._lens, self._lens_tensor = self._ints("lens", t), t
 
     def tensors(self):

@@ -247,3 +247,30 @@ def test_attention_refuses_output_rows_on_one_another():
         return st == C.FA_ERR_INVALID and "stride of 0" in lib.fa_last_error(None).decode()
     assert refused(4, 2, 0, 128, 64) and refused(4, 2, 512, 0, 64) and refused(4, 2, 512, 128, 0)
     assert not refused(4, 2, 512, 128, 64) and not refused(1, 1, 64, 0, 0)
+
+
+def test_scale_past_fp32_is_refused():
+    """The kernels hold scale log2 e: a finite scale whose product is none would make every score infinite or NaN."""
+    from flashact_b200 import _capi as C
+    from flashact_b200.build import build
+    lib = C.load_library(build())
+    c = C.FaKv8(16, 16, 16, 16, 1, 1, 1, 64, 128, 64)
+    r = C.FaRows(16, 64, 64, 64)
+
+    def refused(scale):
+        st = lib.fa_kv8_attention(ctypes.byref(c), 0, 1, 1, ctypes.byref(r), C.FA_DT_BF16, 16, None, None, 1, scale, 0,
+                                  ctypes.byref(r), None, 0, None)
+        return st == C.FA_ERR_INVALID and "finite" in lib.fa_last_error(None).decode()
+    assert refused(2.9e38) and refused(-2.9e38) and refused(float("inf")) and refused(float("nan"))
+    assert not refused(2.3e38) and not refused(-1.0) and not refused(0.0)
+
+
+def test_lens_must_be_a_tensor():
+    from flashact_b200 import FlashActError, Kv8Cache
+    c = Kv8Cache.__new__(Kv8Cache)
+    c._lens, c._lens_tensor = 16, "as it was"
+    with pytest.raises(FlashActError):
+        c.lens = None
+    assert (c._lens, c.lens) == (16, "as it was")
+    with pytest.raises(FlashActError):
+        Kv8Cache.from_tensors(*[torch.zeros(()) for _ in range(4)])
