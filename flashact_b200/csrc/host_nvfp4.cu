@@ -243,15 +243,15 @@ extern "C" fa_status fa_nvfp4_linear(const void* x, fa_dtype dtype, int M, int K
       reinterpret_cast<uintptr_t>(tensor_scale) % 4 || reinterpret_cast<uintptr_t>(bias) % 4)
     return fail(nullptr, FA_ERR_INVALID, "x must be 16-byte aligned, the codes 8-byte, the others to their type");
   if (M == 0) return FA_OK;
+  fa_status st = check_pointers({{"x", x}, {"packed", packed}, {"block_scale", block_scale}, {"tensor_scale", tensor_scale}, {"y", y}});
+  if (st != FA_OK) return st;
+  if (bias && (st = check_pointers({{"bias", bias}})) != FA_OK) return st;
   // blocks write rows of y while others still read x
   const auto at = [](const void* p, long long elements) { return (long long)reinterpret_cast<uintptr_t>(p) + 2 * elements; };
   for (int i = 0; i < M; ++i)
     for (int j = 0; j < M; ++j)
       if (at(x, i * ldx) < at(y, j * ldy + N) && at(y, j * ldy) < at(x, i * ldx + K))
         return fail(nullptr, FA_ERR_INVALID, "y overlaps x");
-  fa_status st = check_pointers({{"x", x}, {"packed", packed}, {"block_scale", block_scale}, {"tensor_scale", tensor_scale}, {"y", y}});
-  if (st != FA_OK) return st;
-  if (bias && (st = check_pointers({{"bias", bias}})) != FA_OK) return st;
   int dev = 0, sms = 148;
   FA_CUDA(nullptr, cudaGetDevice(&dev));
   FA_CUDA(nullptr, cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));

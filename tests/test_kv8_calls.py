@@ -216,20 +216,32 @@ def test_values_past_32_bits(require_gpu):
             assert p.min() > 1e-9 and ((got[b, 0, h] - o).abs() <= tol).all(), (b, h, p.tolist(), ((got[b, 0, h] - o).abs() / tol).max().item())
 
 
-def test_linear_refuses_an_output_over_its_input():
-    """Blocks write y while others read x. Rows beside each other in one buffer do not overlap."""
-    from flashact_b200 import _capi as C
-    from flashact_b200.build import build
-    lib = C.load_library(build())
+@pytest.mark.gpu
+def test_linear_refuses_an_output_over_its_input(require_gpu):
+    """Blocks write y while others read x. Columns beside each other in one buffer do not overlap."""
+    from flashact_b200 import FlashActError, _capi as C
+    from flashact_b200.quant import nvfp4_linear
+    from tests.test_nvfp4_linear import check_linear
+    lib = C.load_library()
+    g = torch.Generator().manual_seed(5)
+    w = (torch.randint(0, 256, (64, 32), generator=g, dtype=torch.uint8).cuda(),
+         torch.randint(0, 100, (64, 4), generator=g, dtype=torch.uint8).cuda(), torch.tensor([1e-2], device="cuda"))
+    x = torch.randn(4, 64, generator=g).to(BF).cuda()
+    with pytest.raises(FlashActError, match="overlaps"):
+        nvfp4_linear(x, *w, out=x)
+    buf = torch.zeros(4, 128, dtype=BF, device="cuda")
+    buf[:, :64] = x
 
-    def call(x, y, M, K, ldx, N, ldy):
-        st = lib.fa_nvfp4_linear(x, C.FA_DT_BF16, M, K, ldx, 1 << 20, 1 << 20, 1 << 20, None, N, y, ldy, None)
-        return st == C.FA_ERR_INVALID and "overlaps" in lib.fa_last_error(None).decode()
-    assert call(4096, 4096, 1, 64, 64, 64, 64) and call(4096, 4096, 16, 64, 64, 64, 64)
-    assert call(4096, 4096 + 2 * 63, 1, 64, 64, 8, 8) and not call(4096, 4096 + 2 * 64, 1, 64, 64, 8, 8)
-    assert call(4096, 4096 - 2 * 7, 1, 64, 64, 8, 8) and not call(4096, 4096 - 2 * 8, 1, 64, 64, 8, 8)
-    # columns 0..63 are x, 64..95 are y, of rows of 96
-    assert not call(4096, 4096 + 2 * 64, 16, 64, 96, 32, 96) and call(4096, 4096 + 2 * 64, 16, 64, 96, 33, 96)
+    def call(y, N, ldy):
+        return lib.fa_nvfp4_linear(buf.data_ptr(), C.FA_DT_BF16, 4, 64, 128, w[0].data_ptr(), w[1].data_ptr(), w[2].data_ptr(), None, N,
+                                   buf.data_ptr() + 2 * y, ldy, torch.cuda.current_stream().cuda_stream)
+    for y, N, ldy in ((0, 64, 128), (63, 64, 128), (64 + 3 * 128, 64, 64), (65, 64, 128), (10, 8, 128)):
+        overlaps = any(y + j * ldy < i * 128 + 64 and i * 128 < y + j * ldy + N for i in range(4) for j in range(4))
+        if overlaps:  # the others lie inside the buffer only where the next line says so
+            assert call(y, N, ldy) == C.FA_ERR_INVALID, (y, N, ldy)
+    assert call(64, 64, 128) == C.FA_OK
+    check_linear(buf[:, 64:].contiguous(), x, *w)
+    assert torch.equal(buf[:, :64], x)
 
 
 def test_attention_refuses_output_rows_on_one_another():
