@@ -74,7 +74,7 @@ class Kv8Cache:
         self._c = C.FaKv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), b, layers, heads, d, cap,
                           self.block)
         self._ref = ctypes.byref(self._c)
-        self._ws = {}  # workspace bytes of the shapes asked for
+        self._ws = {}  # workspace bytes of the last shapes asked for
         self._index, self._lens, self._scale = self.device.index, lens.data_ptr(), d ** -0.5
         self._append, self._attention = self.lib.fa_kv8_append, self.lib.fa_kv8_attention
 
@@ -169,6 +169,8 @@ class Kv8Cache:
         if need is None:
             n = ctypes.c_size_t()
             self._check(self.lib.fa_kv8_attention_workspace(self._ref, tokens, q_heads, max_len, _byref(n)))
+            if len(self._ws) >= 64:  # a caller whose max_len follows each step
+                self._ws.clear()
             need = self._ws[tokens, q_heads, max_len] = n.value
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._check(self._attention(

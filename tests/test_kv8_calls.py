@@ -286,3 +286,14 @@ def test_lens_must_be_a_tensor():
     assert (c._lens, c.lens) == (16, "as it was")
     with pytest.raises(FlashActError):
         Kv8Cache.from_tensors(*[torch.zeros(()) for _ in range(4)])
+
+
+@pytest.mark.gpu
+def test_exact_max_len_of_each_step_is_not_kept(require_gpu):
+    """A decoder that passes each step's length as max_len: what the cache remembers stays small."""
+    from flashact_b200 import Kv8Cache
+    c = Kv8Cache(1, 1, 1, 64, 512)
+    q = torch.zeros(1, 1, 1, 64, dtype=BF, device="cuda")
+    for n in range(1, 300):
+        c.attend(0, q, max_len=n)
+    assert len(c._ws) <= 64
