@@ -174,12 +174,12 @@ extern "C" fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, in
   const unsigned limit = spin_limit.load(std::memory_order_relaxed);
   a.fault_split = fault_split.load(std::memory_order_relaxed);
   a.spin_limit = limit ? (int)std::min(limit, fa::kSpinLimit) : (int)fa::kSpinLimit;
-  a.k = c->k, a.v = c->v, a.ks = c->k_scale, a.vs = c->v_scale;
+  a.ks = c->k_scale, a.vs = c->v_scale;
   a.q = q->ptr, a.out = out->ptr;
   a.qb = q->batch, a.qt = q->token, a.qh = q->head;
   a.ob = out->batch, a.ot = out->token, a.oh = out->head;
   a.mask = Mask{lens, q_lens, prefix, causal != 0, tokens, top};
-  a.layers = c->layers, a.layer = layer, a.heads = c->heads, a.group = q_heads / c->heads, a.dim = c->head_dim, a.cap = c->capacity;
+  a.layers = c->layers, a.layer = layer, a.heads = c->heads, a.group = q_heads / c->heads, a.dim = c->head_dim;
   a.blocks = c->capacity / c->block, a.block_log2 = __builtin_ctz(c->block), a.half = dtype == FA_DT_F16;
   a.q_wide = reinterpret_cast<uintptr_t>(q->ptr) % 16 == 0 && q->batch % 8 == 0 && q->token % 8 == 0 && q->head % 8 == 0;
   a.o_wide = reinterpret_cast<uintptr_t>(out->ptr) % 8 == 0 && out->batch % 4 == 0 && out->token % 4 == 0 && out->head % 4 == 0;

@@ -35,11 +35,8 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 
 // bf16: a code's bits in place are its value times 2^-126, the scale goes in times 2^100, the rest at the end. fp16: values as they
 // are; code times scale lies between 2^-10 and 2688.
-template <bool HALF>
-struct Fmt {
-  static constexpr float SCALE = HALF ? 1.0f : 1.2676506002282294e30f;  // 2^100
-  static constexpr float UNIT = HALF ? 1.0f : 67108864.0f;              // 2^26
-};
+constexpr float kScaleUp = 1.2676506002282294e30f;  // 2^100
+constexpr float kRest = 67108864.0f;                // 2^26
 
 // Two codes of a word as the two halves: bf16 codes I and I + 4 (bits put in place), fp16 codes 2 I and 2 I + 1 (one conversion,
 // measured 2.2 cycles against 8 for the bits; there is none to bf16).
@@ -71,7 +68,7 @@ __device__ __forceinline__ void factors(uint32_t two, uint32_t (&f)[N]) {
   uint32_t v = e4m3_lo_f16x2(two);
   if constexpr (!HALF) {
     const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v));
-    const __nv_bfloat162 y = __floats2bfloat162_rn(x.x * Fmt<false>::SCALE, x.y * Fmt<false>::SCALE);
+    const __nv_bfloat162 y = __floats2bfloat162_rn(x.x * kScaleUp, x.y * kScaleUp);
     v = *reinterpret_cast<const uint32_t*>(&y);
   }
   f[0] = __byte_perm(v, 0, 0x1010);
@@ -200,7 +197,7 @@ __global__ void __launch_bounds__(LW * 32, 2) linear_kernel(const LinArgs a) {
       part[w][r * 16 + g + 8][m * 8 + 2 * t + 1] = acc[r][m][3];
     }
   __syncthreads();
-  const float unit = __ldg(a.ts) * Fmt<HALF>::UNIT;
+  const float unit = __ldg(a.ts) * (HALF ? 1.0f : kRest);
   for (int i = threadIdx.x; i < 16 * RT * a.M; i += LW * 32) {
     const int r = i % (16 * RT), m = i / (16 * RT), n = row0 + r;
     if (n >= a.N) continue;

@@ -6,13 +6,12 @@ namespace fa {
 namespace kv8 {
 
 struct AttnArgs {
-  const unsigned char *k, *v;
   const float *ks, *vs;
   const void* q;
   void* out;
   long long qb, qt, qh, ob, ot, oh;  // element strides: batch, token, head
   Mask mask;
-  int layers, layer, heads, group, dim, cap, blocks, block_log2, half;  // half: fp16 queries (else bf16)
+  int layers, layer, heads, group, dim, blocks, block_log2, half;  // half: fp16 queries (else bf16)
   int q_wide, o_wide;  // rows of queries are 16-byte, of the output 8-byte aligned
   float scale_log2;  // score scale * log2(e)
   uint32_t group_mul;  // ceil(2^32 / group): token of a row without a division

@@ -181,7 +181,7 @@ FA_API fa_status fa_kv8_append(const fa_kv8* c, int layer, int rows, const fa_ro
 
 /* The values of the cache as [batch][layers][rows][heads * head_dim] in `dtype` (f32, bf16: exact where scales are
  * powers of two; f16), k and v 16-byte aligned: the layout fa_bind_prefix_kv takes. lens device int32
- * [batch]; rows at and behind lens[b] are zero. */
+ * [batch]; rows at and behind lens[b] are zero. batch x layers is at most 65535. */
 FA_API fa_status fa_kv8_read(const fa_kv8* c, const int* lens, int rows, void* k, void* v, fa_dtype dtype,
                              fa_stream stream);
 
