@@ -60,26 +60,43 @@ fa_status byte_map(CUtensorMap* m, const void* base, uint64_t inner, uint64_t ro
 }
 
 // The kernel and the splits of whole 128-key tiles: the number of splits with the least time by a model of measured parts (B200, us).
-// A CTA of kv8_attn_few.cu (two on an SM) pays about 4 for its start and end, and for a tile its bytes at the SM's share of the
-// memory (45 GB/s for an SM, 6.5 TB/s for all; lengths are mostly below max_len, hence 0.85). A CTA of kv8_attn_rows.cu (one on an
-// SM) pays about 10, its queries' parts and the join of the splits, and 1.9 (fp16 2.1) for a tile. Up to eight splits are a cluster (0.7);
-// more need the merge kernel (3).
-Plan make_plan(const fa_kv8* c, int tokens, int q_heads, int max_len, int sms) {
+// Waves come from what the device has room for, in blocks or in whole clusters of the split's size (a cluster of 8 blocks that fill an SM
+// leaves many SMs idle). A wave costs its start and end and its tiles. Up to 16 rows: 6 or 7 (16 rows), a tile 1.05 or 1.2 (a chain of
+// latencies, whatever head_dim); where many are read at once their bytes at the memory's rate are the longer part (lengths are mostly below max_len,
+// hence 0.85), and a quarter of the shorter one is not hidden. 128 rows: 12, a tile 2.2 at head_dim 256 and 1.7 below. fp16 has 1.1 and 1.3
+// times that a tile. Then the join: in a cluster 0.5, and with 128 rows 8 / n
+// (its blocks share the output) + 0.5 n; by the merge kernel, which reads n sums a row, 1 + 0.4 n, and with 128 rows 11 + 0.2 n at
+// head_dim 256, less below.
+// Over 66 shapes (1 to 64 observations, 1 to 968 tokens, 300 to 32768 keys, head_dim 64 to 256, both types) the planned number is within 7% of
+// the best of 18 tried, in 58 of them within 3%.
+Plan make_plan(const fa_kv8* c, int tokens, int q_heads, int max_len, int device, bool half) {
   Plan p;
   const long long all = (long long)tokens * (q_heads / c->heads);
   p.rows = all <= 8 ? 8 : all <= 16 ? 16 : 128;
   p.tiles = (int)((all + p.rows - 1) / p.rows);
   const bool few = p.rows < 128;
-  const int chunks = std::max(1, (max_len + 127) / 128), slots = (few ? 2 : 1) * sms;
+  const int chunks = std::max(1, (max_len + 127) / 128);
   const long long base = (long long)c->batch * c->heads * p.tiles;
   const double mb = 256e-6 * c->head_dim;  // a tile's bytes, in MB
+  const double fix = few ? (p.rows == 8 ? 6 : 7) : 12;
+  const double lat = few ? (p.rows == 8 ? 1.05 : 1.2) * (half ? 1.1 : 1) : (c->head_dim > 128 ? 2.2 : 1.7) * (half ? 1.3 : 1);
+  const auto resident = [&](int n) {
+    const int got = device < 0 ? 0 : few ? kv8_resident_few(p.rows, half, c->head_dim, device, n) : kv8_resident_rows(half, c->head_dim, device, n);
+    return got > 0 ? got : std::max(1, (few && c->head_dim <= 128 ? 2 : 1) * 148 / n);
+  };
+  int fit[9];
+  for (int n = 1; n <= 8 && n <= chunks; ++n) fit[n] = resident(n);
   double best = 1e300;
   p.nsplit = 1;
   for (int n = 1; n <= 64 && n <= chunks; ++n) {
     const int each = (chunks + n - 1) / n;
-    const double ctas = (double)base * n, waves = std::ceil(ctas / slots);
-    const double tile = few ? std::max(mb / 0.045, std::min(ctas, (double)slots) * mb * (0.85 / 6.5)) : 2.0;
-    const double cost = waves * ((few ? 4 : 10) + each * tile) + (n > 8 ? 3 + 0.1 * n : n > 1 ? 0.7 : 0);
+    const bool cluster = n <= 8;
+    const double groups = cluster ? (double)base : (double)base * n, room = fit[cluster ? n : 1];
+    const double active = std::min(groups, room) * (cluster ? n : 1);
+    const double chain = each * lat, bytes = few ? active * chunks / n * mb * (0.85 / 6.5) : 0;
+    double join = n > 8 ? 1 + 0.4 * n : n > 1 ? 0.5 : 0;
+    if (!few) join = n > 8 ? 11 * c->head_dim / 256.0 + 0.2 * n : 8.0 / n + 0.5 * n;
+    const double cost = std::ceil(groups / room) * (fix + std::max(chain, bytes) + 0.25 * std::min(chain, bytes)) + join;
     if (cost < best) best = cost, p.nsplit = n;
   }
   p.split_chunks = (chunks + p.nsplit - 1) / p.nsplit;
@@ -105,22 +122,14 @@ fa_status attn_check(const fa_kv8* c, int tokens, int q_heads, int max_len) {
 std::atomic<int> fault_split{-1};
 std::atomic<unsigned> spin_limit{0};
 
-// SMs of the current device; 148 where there is none, so that a workspace can be sized anywhere.
-int sm_count(int* device = nullptr) {
-  static std::atomic<int> known[64];
-  int dev = 0, n = 0;
+// The current device; -1 where there is none, so that a workspace can be asked for anywhere.
+int current_device() {
+  int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
-    return 148;
+    return -1;
   }
-  if (device) *device = dev;
-  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();
-    return 148;
-  }
-  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
-  return n;
+  return dev;
 }
 
 }  // namespace
@@ -134,8 +143,11 @@ extern "C" fa_status fa_kv8_attention_workspace(const fa_kv8* c, int tokens, int
   fa_status st = attn_check(c, tokens, q_heads, max_len);
   if (st != FA_OK) return st;
   if (!bytes) return fail(nullptr, FA_ERR_INVALID, "null bytes");
-  const Plan p = make_plan(c, std::max(1, tokens), q_heads, max_len ? max_len : c->capacity, sm_count());
-  *bytes = p.part_bytes + p.ml_bytes;
+  *bytes = 0;
+  for (const bool half : {false, true}) {  // for queries of either type
+    const Plan p = make_plan(c, std::max(1, tokens), q_heads, max_len ? max_len : c->capacity, current_device(), half);
+    *bytes = std::max(*bytes, p.part_bytes + p.ml_bytes);
+  }
   return FA_OK;
 }
 
@@ -158,8 +170,8 @@ extern "C" fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, in
     return fail(nullptr, FA_ERR_INVALID, "rows of the output lie on one another (a stride of 0)");
   if (tokens == 0) return FA_OK;
   const int top = max_len ? max_len : c->capacity;
-  int device = 0;
-  const Plan p = make_plan(c, tokens, q_heads, top, sm_count(&device));
+  const int device = current_device();
+  const Plan p = make_plan(c, tokens, q_heads, top, device, dtype == FA_DT_F16);
   if (workspace_bytes < p.part_bytes + p.ml_bytes)
     return fail(nullptr, FA_ERR_INVALID, "workspace of %zu bytes, %zu are needed", workspace_bytes, p.part_bytes + p.ml_bytes);
   if (p.part_bytes && reinterpret_cast<uintptr_t>(workspace) % 16)

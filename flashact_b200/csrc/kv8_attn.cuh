@@ -59,3 +59,6 @@ __device__ __forceinline__ void store16(void* p, long long i, float x, int half)
 // The kernels: up to 16 query rows of a key head (kv8_attn_few.cu), and 128 at a time (kv8_attn_rows.cu).
 fa_status kv8_launch_few(const fa::kv8::AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s);
 fa_status kv8_launch_rows(const fa::kv8::AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s);
+// Clusters of n blocks of the kernel for such a call (n = 1: blocks) that the current device has room for at once; 0 if that is not known.
+int kv8_resident_few(int rows, bool half, int dim, int device, int n);
+int kv8_resident_rows(bool half, int dim, int device, int n);

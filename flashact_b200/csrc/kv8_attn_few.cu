@@ -434,6 +434,10 @@ fa_status launch(const AttnArgs& a, int batch, const CUtensorMap& km, const CUte
   constexpr int SMEM = Cfg<R, HALF, MT>::SMEM;
   return kv8_launch<few_kernel<R, HALF, MT>>(a, batch, THREADS, SMEM, km, vm, s);
 }
+template <int R, bool HALF, int MT>
+int resident(int device, int n) {
+  return kv8_resident<few_kernel<R, HALF, MT>>(device, n, THREADS, Cfg<R, HALF, MT>::SMEM, Cfg<R, HALF, MT>::CTAS);
+}
 template <int R>
 fa_status launch_rows(const AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
   if (a.dim <= 128) return a.half ? launch<R, true, 1>(a, batch, km, vm, s) : launch<R, false, 1>(a, batch, km, vm, s);
@@ -444,4 +448,13 @@ fa_status launch_rows(const AttnArgs& a, int batch, const CUtensorMap& km, const
 
 fa_status kv8_launch_few(const AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
   return a.rows == 8 ? launch_rows<8>(a, batch, km, vm, s) : launch_rows<16>(a, batch, km, vm, s);
+}
+
+int kv8_resident_few(int rows, bool half, int dim, int device, int n) {
+  if (rows == 8) {
+    if (dim <= 128) return half ? resident<8, true, 1>(device, n) : resident<8, false, 1>(device, n);
+    return half ? resident<8, true, 2>(device, n) : resident<8, false, 2>(device, n);
+  }
+  if (dim <= 128) return half ? resident<16, true, 1>(device, n) : resident<16, false, 1>(device, n);
+  return half ? resident<16, true, 2>(device, n) : resident<16, false, 2>(device, n);
 }

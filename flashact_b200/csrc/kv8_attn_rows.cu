@@ -440,9 +440,19 @@ fa_status launch(const AttnArgs& a, int batch, const CUtensorMap& km, const CUte
   return kv8_launch<rows_kernel<HALF, MT>>(a, batch, THREADS, SMEM, km, vm, s);
 }
 
+template <bool HALF, int MT>
+int resident(int device, int n) {
+  return kv8_resident<rows_kernel<HALF, MT>>(device, n, THREADS, Cfg<HALF, MT>::SMEM, 1);
+}
+
 }  // namespace
 
 fa_status kv8_launch_rows(const AttnArgs& a, int batch, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
   if (a.dim <= 128) return a.half ? launch<true, 1>(a, batch, km, vm, s) : launch<false, 1>(a, batch, km, vm, s);
   return a.half ? launch<true, 2>(a, batch, km, vm, s) : launch<false, 2>(a, batch, km, vm, s);
+}
+
+int kv8_resident_rows(bool half, int dim, int device, int n) {
+  if (dim <= 128) return half ? resident<true, 1>(device, n) : resident<false, 1>(device, n);
+  return half ? resident<true, 2>(device, n) : resident<false, 2>(device, n);
 }

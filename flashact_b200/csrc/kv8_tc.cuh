@@ -359,6 +359,40 @@ __device__ __forceinline__ int produce(unsigned char* ring, uint64_t* full, uint
 }  // namespace kv8
 }  // namespace fa
 
+// Clusters of n blocks of a kernel (n = 1: blocks) that `device`, the current one, has room for at once; asked once a kernel, size and
+// device. The parts of the chip that a cluster may not span leave some of it idle, differently for each size. The runtime counts a kernel that
+// allocates tensor memory as one block to an SM; `ctas` fit by registers, shared and tensor memory, and do run together. 0: not known.
+template <auto kernel>
+static int kv8_resident(int device, int n, int threads, int smem, int ctas) {
+  static std::atomic<int> known[64][9];
+  std::atomic<int>& at = known[device & 63][n];
+  int got = at.load(std::memory_order_relaxed);
+  if (got > 0) return got;
+  int sms = 0, blocks = 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(n);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = n;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, smem);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  if (e == cudaSuccess && n > 1) e = cudaOccupancyMaxActiveClusters(&got, kernel, &cfg);
+  if (n == 1) got = blocks * sms;
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (blocks < ctas) got = got / std::max(1, blocks) * ctas;
+  at.store(got, std::memory_order_relaxed);
+  return got;
+}
+
 template <auto kernel>
 static fa_status kv8_launch(const fa::kv8::AttnArgs& a, int batch, int threads, int smem, const CUtensorMap& km,
                             const CUtensorMap& vm, cudaStream_t s) {

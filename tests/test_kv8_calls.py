@@ -297,3 +297,16 @@ def test_exact_max_len_of_each_step_is_not_kept(require_gpu):
     for n in range(1, 300):
         c.attend(0, q, max_len=n)
     assert len(c._ws) <= 64
+
+
+def test_splits_fit_the_kernel_that_runs():
+    """Two tokens of 8 query heads at head_dim 256 are blocks that fill an SM: four observations of a long cache are split into no more
+    of them than there are SMs (148 where no device is), not into two to an SM."""
+    from flashact_b200 import _capi as C
+    from flashact_b200.build import build
+    lib = C.load_library(build())
+    n = ctypes.c_size_t()
+    c = C.FaKv8(16, 16, 16, 16, 4, 1, 1, 256, 1 << 14, 64)
+    assert lib.fa_kv8_attention_workspace(ctypes.byref(c), 2, 8, 0, ctypes.byref(n)) == C.FA_OK
+    splits = n.value // (4 * 16 * (256 * 4 + 8))  # observations x rows x (sums, maximum and sum)
+    assert 8 < splits and 4 * splits <= 148
