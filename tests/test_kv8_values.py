@@ -101,3 +101,20 @@ def test_loud_values_of_faint_keys(require_gpu, T, H, D, dtype, louder):
         got = ref.to_cache([n]).attend(0, q.cuda(), scale=2.0, causal=False)
         want, tol = attend(ref, 0, q, [n], scale=2.0, causal=False)
         check(got, want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("T,H,heads", [(2, 8, 1), (3, 3, 1), (1, 32, 2), (5, 6, 2), (16, 1, 1)])
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("cap,lens", [(128, [100, 3]), (1024, [968, 301]), (1 << 15, [20000, 130])], ids=["one", "cluster", "merge"])
+def test_nine_to_sixteen_rows(require_gpu, T, H, heads, D, cap, lens, dtype):
+    """9 to 16 rows of a key head: one split, splits joined in a cluster and by the merge; prefix masks and padded queries."""
+    assert 9 <= T * H // heads <= 16
+    q_lens, prefix = [T, max(1, T - 1)], [7, lens[1]]
+    ref = random_ref(2, 1, heads, D, cap, 128, D + T)
+    q = _q((2, T, H, D), dtype, T)
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    got = ref.to_cache(lens).attend(0, q.cuda(), q_lens=dev(q_lens), prefix=dev(prefix)).cpu()
+    want, tol = attend(ref, 0, q, lens, q_lens=q_lens, prefix=prefix)
+    check(got, want, tol)
