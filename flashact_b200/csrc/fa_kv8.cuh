@@ -3,8 +3,11 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <initializer_list>
+#include <utility>
+
 #include "fa_ptx.cuh"
-#include "host_common.cuh"
+#include "host_base.cuh"
 
 namespace fa {
 namespace kv8 {

@@ -1,24 +1,12 @@
 // Host-side pieces shared by the model engines behind the C ABI: the handle, error reporting,
 // device allocation, weight staging / row-gather packing, and TMA descriptor builders.
 #pragma once
-#include <cudaTypedefs.h>
-#include <cuda_fp8.h>
-#include <cuda_runtime.h>
-
-#include <algorithm>
-#include <cmath>
-#include <cstdarg>
-#include <cstdio>
-#include <cstdlib>
-#include <cstring>
 #include <mutex>
-#include <string>
 #include <vector>
 
-#include "../../include/flashact.h"
 #include "fa_pi05.cuh"
+#include "host_base.cuh"
 
-using bf16 = __nv_bfloat16;
 using fa::pi05::Params;
 using fa::GemmUnit;
 using fa::AttnUnit;
@@ -79,8 +67,6 @@ struct fa_handle {
   Ma2State* ma2 = nullptr;  // MolmoAct2 engine state (FA_MODEL_MOLMOACT2 handles)
 };
 
-extern thread_local std::string g_create_err;
-
 static inline fa_status fail(fa_handle* h, fa_status st, const char* fmt, ...) {
   char buf[512];
   va_list ap;
@@ -90,13 +76,6 @@ static inline fa_status fail(fa_handle* h, fa_status st, const char* fmt, ...) {
   if (h) h->err = buf; else g_create_err = buf;
   return st;
 }
-#define FA_CUDA(h, call)                                                                        \
-  do {                                                                                          \
-    cudaError_t e_ = (call);                                                                    \
-    if (e_ != cudaSuccess) return fail(h, FA_ERR_CUDA, "%s: %s (%s:%d)", #call, cudaGetErrorString(e_), \
-                                       __FILE__, __LINE__);                                     \
-  } while (0)
-
 template <class T>
 static inline fa_status dalloc(fa_handle* h, T** out, size_t count) {
   void* p = nullptr;
@@ -141,7 +120,6 @@ static __global__ void rowmap_kernel(const unsigned char* keep, int src_rows, in
     if (kb[r]) rowmap[(size_t)b * src_rows + pos++] = r;
   if (t == nt - 1) counts[b] = pos;
 }
-
 
 // Builds the row map of a masked bind on `stream` (into the handle's reusable buffers) and
 // returns the kept-row counts on the host (the bind plans its attention work from them).
@@ -191,8 +169,6 @@ static inline int l2_ahead_layers() {
   return e ? std::max(0, std::min(4, atoi(e))) : 0;
 }
 
-static size_t dtype_size(fa_dtype t) { return t == FA_DT_F32 ? 4 : 2; }
-
 __device__ __forceinline__ float load_as_float(const void* p, size_t i, int dt) {
   if (dt == FA_DT_F32) return reinterpret_cast<const float*>(p)[i];
   if (dt == FA_DT_BF16) return __bfloat162float(reinterpret_cast<const bf16*>(p)[i]);
@@ -216,11 +192,6 @@ __device__ __forceinline__ float e2m1_value(unsigned v) {
   const unsigned e = (v >> 1) & 3u, m = v & 1u;
   const float mag = e == 0 ? 0.5f * (float)m : (1.0f + 0.5f * (float)m) * (float)(1u << (e - 1));
   return (v & 8u) ? -mag : mag;
-}
-__device__ __forceinline__ float e4m3_value(unsigned char c) {
-  __nv_fp8_e4m3 f;
-  f.__x = c;
-  return (float)f;
 }
 static __global__ void pack_rows_kernel(PackSrc s, const int2* rowmap, bf16* dst, int R, int K, int L) {
   const size_t total = (size_t)L * R * K;
@@ -269,17 +240,6 @@ static __global__ void to_f32_kernel(const void* src, int dt, float* dst, size_t
 static inline int round_up(int a, int b) { return (a + b - 1) / b * b; }
 
 // ------------------------------------------------------------------ TMA descriptors
-static inline PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  if (!fn) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  }
-  return fn;
-}
 // 3D bf16 map viewing a row-major [rows][K] array as [K/64 atoms][rows][64]: one box
 // {64, box_rows, box_atoms} lands in shared memory as box_atoms consecutive 128B-swizzled atoms.
 // 2D bf16 map over a row-major [rows][K] matrix: boxes of box_k x box_rows (box_k x 2 bytes = 128 for
@@ -381,7 +341,6 @@ static inline fa_status pack_matrix(fa_handle* h, const std::vector<int2>& rowma
   FA_CUDA(h, cudaGetLastError());
   return FA_OK;
 }
-
 
 // MolmoAct2 engine (host_ma2.cu), reached through the C ABI's model dispatch.
 fa_status ma2_create(const fa_config& cfg, int device, fa_handle* h);
