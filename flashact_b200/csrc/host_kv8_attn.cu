@@ -63,12 +63,11 @@ fa_status byte_map(CUtensorMap* m, const void* base, uint64_t inner, uint64_t ro
 // Waves come from what the device has room for, in blocks or in whole clusters of the split's size (a cluster of 8 blocks that fill an SM
 // leaves many SMs idle). A wave costs its start and end and its tiles. Up to 16 rows: 6 or 7 (16 rows), a tile 1.05 or 1.2 (a chain of
 // latencies, whatever head_dim); where many are read at once their bytes at the memory's rate are the longer part (lengths are mostly below max_len,
-// hence 0.85), and a quarter of the shorter one is not hidden. 128 rows: 12, a tile 2.2 at head_dim 256 and 1.7 below. fp16 has 1.1 and 1.3
-// times that a tile. Then the join: in a cluster 0.5, and with 128 rows 8 / n
-// (its blocks share the output) + 0.5 n; by the merge kernel, which reads n sums a row, 1 + 0.4 n, and with 128 rows 11 + 0.2 n at
-// head_dim 256, less below.
-// Over 66 shapes (1 to 64 observations, 1 to 968 tokens, 300 to 32768 keys, head_dim 64 to 256, both types) the planned number is within 7% of
-// the best of 18 tried, in 58 of them within 3%.
+// hence 0.85), and a quarter of the shorter one is not hidden. 128 rows: 12, a tile 1.7 at head_dim 64 to 2.6 at 256. fp16 has 1.1 and 1.35
+// times that a tile. Then the join: in a cluster 1 to 2.4, with 128 rows, whose sums are many, 2 to 5; by the merge kernel, where a warp reads its row's
+// sums split by split, 2 and 0.29 to 0.4 a split, with 128 rows 0.8 to 3 and 0.16 to 0.36 a split.
+// Over 86 shapes (1 to 100 observations, 1 to 968 tokens, 156 to 32768 keys, head_dim 64 to 256, both types) the planned number is within 10% of
+// the best of 18 tried, in 79 of them within 3%.
 Plan make_plan(const fa_kv8* c, int tokens, int q_heads, int max_len, int device, bool half) {
   Plan p;
   const long long all = (long long)tokens * (q_heads / c->heads);
@@ -79,7 +78,7 @@ Plan make_plan(const fa_kv8* c, int tokens, int q_heads, int max_len, int device
   const long long base = (long long)c->batch * c->heads * p.tiles;
   const double mb = 256e-6 * c->head_dim;  // a tile's bytes, in MB
   const double fix = few ? (p.rows == 8 ? 6 : 7) : 12;
-  const double lat = few ? (p.rows == 8 ? 1.05 : 1.2) * (half ? 1.1 : 1) : (c->head_dim > 128 ? 2.2 : 1.7) * (half ? 1.3 : 1);
+  const double lat = few ? (p.rows == 8 ? 1.05 : 1.2) * (half ? 1.1 : 1) : (1.4 + 0.0047 * c->head_dim) * (half ? 1.35 : 1);
   const auto resident = [&](int n) {
     const int got = device < 0 ? 0 : few ? kv8_resident_few(p.rows, half, c->head_dim, device, n) : kv8_resident_rows(half, c->head_dim, device, n);
     return got > 0 ? got : std::max(1, (few && c->head_dim <= 128 ? 2 : 1) * 148 / n);
@@ -94,8 +93,8 @@ Plan make_plan(const fa_kv8* c, int tokens, int q_heads, int max_len, int device
     const double groups = cluster ? (double)base : (double)base * n, room = fit[cluster ? n : 1];
     const double active = std::min(groups, room) * (cluster ? n : 1);
     const double chain = each * lat, bytes = few ? active * chunks / n * mb * (0.85 / 6.5) : 0;
-    double join = n > 8 ? 1 + 0.4 * n : n > 1 ? 0.5 : 0;
-    if (!few) join = n > 8 ? 11 * c->head_dim / 256.0 + 0.2 * n : 8.0 / n + 0.5 * n;
+    const double d = c->head_dim;
+    const double join = n > 8 ? (few ? 2 + n * (0.25 + d / 1700) : 3 * d / 256 + n * (0.1 + d / 1000)) : few ? (n > 1 ? 0.8 + 0.2 * n : 0) : 1 + d / 64;
     const double cost = std::ceil(groups / room) * (fix + std::max(chain, bytes) + 0.25 * std::min(chain, bytes)) + join;
     if (cost < best) best = cost, p.nsplit = n;
   }

@@ -442,7 +442,7 @@ fa_status launch(const AttnArgs& a, int batch, const CUtensorMap& km, const CUte
 
 template <bool HALF, int MT>
 int resident(int device, int n) {
-  return kv8_resident<rows_kernel<HALF, MT>>(device, n, THREADS, Cfg<HALF, MT>::SMEM, 1);
+  return kv8_resident<rows_kernel<HALF, MT>>(device, n, THREADS, Cfg<HALF, MT>::SMEM);
 }
 
 }  // namespace

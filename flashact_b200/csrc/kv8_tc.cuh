@@ -359,16 +359,17 @@ __device__ __forceinline__ int produce(unsigned char* ring, uint64_t* full, uint
 }  // namespace kv8
 }  // namespace fa
 
-// Clusters of n blocks of a kernel (n = 1: blocks) that `device`, the current one, has room for at once; asked once a kernel, size and
-// device. The parts of the chip that a cluster may not span leave some of it idle, differently for each size. The runtime counts a kernel that
-// allocates tensor memory as one block to an SM; `ctas` fit by registers, shared and tensor memory, and do run together. 0: not known.
+// Clusters of n blocks (n = 1: blocks) of `threads` threads and `smem` bytes that `device`, the current one, has room for at once; asked
+// once a kernel, size and device. The parts of the chip that a cluster may not span leave some of it idle, differently for each size. Asked for a
+// kernel without tensor memory: the runtime counts one that allocates it as one block to an SM, while as many run as shared memory has room for
+// (Cfg sees to it that registers and tensor memory do too). 0: not known.
+static __global__ void room_kernel() {}
 template <auto kernel>
-static int kv8_resident(int device, int n, int threads, int smem, int ctas) {
+static int kv8_resident(int device, int n, int threads, int smem) {
   static std::atomic<int> known[64][9];
   std::atomic<int>& at = known[device & 63][n];
-  int got = at.load(std::memory_order_relaxed);
+  int got = at.load(std::memory_order_relaxed), sms = 0;
   if (got > 0) return got;
-  int sms = 0, blocks = 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(n);
   cfg.blockDim = dim3(threads);
@@ -379,16 +380,15 @@ static int kv8_resident(int device, int n, int threads, int smem, int ctas) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, smem);
+  cudaError_t e = cudaFuncSetAttribute(room_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-  if (e == cudaSuccess && n > 1) e = cudaOccupancyMaxActiveClusters(&got, kernel, &cfg);
-  if (n == 1) got = blocks * sms;
+  if (e == cudaSuccess)
+    e = n > 1 ? cudaOccupancyMaxActiveClusters(&got, room_kernel, &cfg) : cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, room_kernel, threads, smem);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
-  if (blocks < ctas) got = got / std::max(1, blocks) * ctas;
+  if (n == 1) got *= sms;
   at.store(got, std::memory_order_relaxed);
   return got;
 }
