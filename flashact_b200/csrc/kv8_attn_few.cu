@@ -301,7 +301,15 @@ __global__ void __launch_bounds__(THREADS, (Cfg<R, HALF, MT>::CTAS))
       if (fl.x | fl.y | fl.z | fl.w) {  // the same in all 128 threads
         float x[2 * R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) x[r] = warp_max(s[r]), x[R + r] = warp_max(s[r] + lv);
+        for (int r = 0; r < R; ++r) x[r] = warp_max(s[r]);
+        if (a.block_log2 >= 5) {  // a warp's 32 keys are of one block
+          const float lw = __shfl_sync(0xffffffffu, lv, 0);
+#pragma unroll
+          for (int r = 0; r < R; ++r) x[R + r] = x[r] + lw;
+        } else {
+#pragma unroll
+          for (int r = 0; r < R; ++r) x[R + r] = warp_max(s[r] + lv);
+        }
         if (lane == 0) {
 #pragma unroll
           for (int r = 0; r < 2 * R; r += 4)

@@ -300,11 +300,11 @@ enum { ERR_FULL = 1, ERR_EMPTY, ERR_S, ERR_SFREE, ERR_P, ERR_PV, ERR_SEEN };
 
 // A bounded wait, as mbar_wait, whose limit stands behind the block's error word (err[1]).
 static __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t phase, volatile int* err, int code) {
-  const uint32_t limit = (uint32_t)err[1];
-  for (uint32_t i = 0; i < limit; ++i) {
+  for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait(bar, phase)) return true;
-    if ((i & 255u) == 255u) {
+    if ((i & 255u) == 0) {
       if (*err) return false;
+      if (i >= (uint32_t)err[1]) break;
       __nanosleep(64);
     }
   }
@@ -319,7 +319,7 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t phase, volatile
 // issued and the products, which the issuing warps put on `drained`; then all its rows are NaN, sums and (maximum, sum). A sum that is NaN
 // goes through each join and the merge, where a sum of 0 would be a split without a key. All threads come here.
 template <int SLOTS>
-__device__ __forceinline__ void give_up(uint64_t* full, int issued, uint64_t* drained, bool issuer, float* o, int pitch, int width,
+static __device__ __noinline__ void give_up(uint64_t* full, int issued, uint64_t* drained, bool issuer, float* o, int pitch, int width,
                                         float* ml, int ml_pitch, int rows) {
   if (issuer) tc_commit_elect(drained);
   if (threadIdx.x == 0) {
