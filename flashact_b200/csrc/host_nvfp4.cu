@@ -13,10 +13,12 @@
 // operands share it: a lane owns PB bytes of codes (one or two scale blocks) of each of its rows, read
 // with one load a turn ahead, and x's pairs follow the order in which the codes come out of a word.
 //
-// Measured: 16 rows by 28672 x 8192 in fp16 55 us (2.4 TB/s), 8 by 32768 x 2048 in bf16 16.4 us (2.3 TB/s), one by 2560 x 1024
-// 2.4 us. The memory's time for the first two is 20 and 6 us. What bounds them is taking the codes apart (8 cycles of a scheduler for
-// a pair of bf16 codes, 2.2 for fp16) with the registers of two warps to a scheduler: of the cycles in which a CTA is there,
-// 44% issue, the rest waits for loads and for results; and the last wave (448 CTAs at 296 places in the first case).
+// Measured in a graph, inputs beyond L2: 16 rows by 28672 x 8192 in fp16 55 us (2.4 TB/s), 8 by 32768 x 2048 in bf16 17.0 us (2.3 TB/s),
+// one by 2560 x 1024 2.3 us. The memory's time for the first two is 20 and 6 us. Two CTAs share an SM at 128 registers (13 to 14 warps at
+// work) and use 35% of the issue slots in the first case, 50% in the second. Between two instructions a warp waits 4.4 and 2.5 cycles for loads (a CTA reads
+// all of x, in the first case as many bytes as of weights, from L2) and 1.6 and 0.8 for results; taking bf16 codes apart (8 cycles of a
+// scheduler for a pair, 2.2 for fp16) keeps the integer pipe 45% busy. The last wave is half empty (448 CTAs at 296 places). The
+// instances of 64 rows of W and wide loads, which large matrices take, hold 56 to 120 bytes a thread in local memory.
 // Weights through a ring in shared memory, and CTAs that stay for several rows of W, took longer than registers loaded a turn ahead.
 #include "fa_kv8.cuh"
 

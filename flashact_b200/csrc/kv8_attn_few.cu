@@ -16,12 +16,13 @@
 //
 // One CTA takes R query rows of a (observation, key head) and a split of the keys in tiles of 128: warp 0 keeps a ring
 // of K and V tiles full, warp 1 issues the products (scores of tile i + 1 before P V of tile i), warps 2..5 turn scores into
-// probabilities. The running maxima (of p and of p vs) move
-// only where one of them grew by more than 2^3, the only case that touches O^T.
+// probabilities. The running maxima (of p and of p vs) move only where one of them grew by more than 2^3, the only case that touches O^T.
 //
-// Bound by the cache's bytes where it is long: one token of 8 observations at 32768 keys of 8 key heads of 128 takes 88 us,
-// 6.1 TB/s. A short cache is a chain of latencies: one observation, 968 keys of one key head of 256, takes 8.2 us (launch 2,
-// start and queries 2, tiles 2, join 1); 64 observations at up to 1736 keys 14.3 us, 3.0 TB/s with two CTAs on an SM.
+// Measured in a graph, inputs beyond L2. Bound by the cache's bytes where it is long: one token of 8 observations at 32768 keys of 8 key heads
+// of 128 takes 86 to 89 us, 6.1 TB/s. A short cache is a chain of latencies: one observation, 968 keys of one key head of 256, takes 7.7 us
+// (launch 2, start and queries 2, tiles 2, join 1), and a tile about 1.05 us whatever its head_dim (1.2 with 16 rows); 64 observations at up to 1736
+// keys 15.3 us, 2.9 TB/s, with two CTAs on an SM and 24% of the issue slots used. 16 rows at head_dim up to 128 need more registers than two
+// CTAs leave them: about 160 bytes a thread are stored in local memory and 300 read.
 // Converting the codes to f16 for the 16-bit matrix instruction took 117, 34 and 29 us: the conversion costs more
 // than the products. The warp-level matrix instruction's 8-bit form is carried out in many steps here and took longer still.
 #include "kv8_tc.cuh"
@@ -32,7 +33,7 @@ using namespace fa;
 using namespace fa::kv8;
 
 constexpr int THREADS = 192;
-constexpr float kPTop = 12.0f;  // log2 of P where p vs = 2^d; with a maximum that lags by up to kLag and kSlack, 2^15.25 (E5M2 ends at 57344)
+constexpr float kPTop = 12.0f;  // log2 of P where p vs = 2^d; with maxima that lag by up to kLag, 2^15 (E5M2 ends at 57344)
 constexpr float kLag = 3.0f, kSlack = 0.25f;
 
 __device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 128;" ::: "memory"); }

@@ -21,12 +21,13 @@
 // the two threads of a row exchange their maxima, those of tile i + 1 while they write P of tile i. The running maxima (of p and of
 // p vs) move only where one of them grew by more than 2^1, the only case that touches O.
 //
-// Measured at head_dim 256 (bf16): a tile takes about 2 us, its products 2560 cycles of that (64 for a score product of K = 32,
+// Measured in a graph at head_dim 256 (bf16): a tile takes 2.2 to 2.6 us, its products 2560 cycles of that (64 for a score product of K = 32,
 // 128 for one of P V); a CTA's start 4 us, 2 of them the queries' parts, its end 5. 16 observations of 50 tokens and 8
-// query heads on one key head at 1018 keys: 26 us (258 TFLOP/s, each product counted once); 4 of 256 tokens in fp16 at up to
-// 4096: 76 us (364). With 16-bit products and converted tiles these took 74 and 222 us. Rows come here from 17 on: a tile of
-// 128 costs the same however many of its rows are used, and kv8_attn_few.cu needs tensor memory columns for each part of
-// each row, enough for 16.
+// query heads on one key head at 1018 keys: 25.7 us (260 TFLOP/s, each product counted once; the tensor cores are busy 16% of it, 35% of the
+// issue slots are used); 4 of 256 tokens in fp16 at up to 4096: 76 us (364; 28% and 39%). With 16-bit products and converted tiles these took 74
+// and 222 us. The fp16 instances hold 24 bytes a thread in local memory. Rows come here from 17 on: a tile of 128 costs the same however
+// many of its rows are used; kv8_attn_few.cu, which gives each part of each row its own columns, is built for 8 and 16 (32 would fit
+// its tensor memory too: 320 columns in bf16 and 448 in fp16 at head_dim 256).
 #include "kv8_tc.cuh"
 
 namespace {
