@@ -89,6 +89,7 @@ class Kv8Cache:
         self._lens, self._lens_tensor = self._ints("lens", t), t
 
     def tensors(self):
+        """The memory that the cache is: k, v, k_scale, v_scale, lens."""
         return self.k, self.v, self.k_scale, self.v_scale, self._lens_tensor
 
     def _check(self, st):

@@ -1,5 +1,9 @@
 """Calls of the 8-bit KV cache and the NVFP4 linear layer at the edges of what their documentation allows."""
 import ctypes
+import os
+import subprocess
+import sys
+import threading
 from types import SimpleNamespace
 
 import pytest
@@ -310,3 +314,71 @@ def test_splits_fit_the_kernel_that_runs():
     assert lib.fa_kv8_attention_workspace(ctypes.byref(c), 2, 8, 0, ctypes.byref(n)) == C.FA_OK
     splits = n.value // (4 * 16 * (256 * 4 + 8))  # observations x rows x (sums, maximum and sum)
     assert 8 < splits and 4 * splits <= 148
+
+
+FIRST = """
+import torch
+from flashact_b200 import Kv8Cache
+from flashact_b200.quant import nvfp4_linear
+BF = torch.bfloat16
+c = Kv8Cache(2, 1, 1, 256, 1 << 14)
+k = torch.randn(2, 300, 1, 256, device="cuda").to(BF)
+q = [torch.randn(2, t, 8, 256, device="cuda").to(dt) for t in (1, 2, 40) for dt in (BF, torch.float16)]
+x, w, bs, ts = torch.ones(1, 64, dtype=BF, device="cuda"), *(torch.zeros(8, n, dtype=torch.uint8, device="cuda") for n in (32, 4)), torch.ones(1, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):  # nothing of the library has run before
+    c.append(0, k, k)
+    c.advance(300)
+    got = [c.attend(0, x) for x in q]
+    v = c.read(300)
+    y = nvfp4_linear(x, w, bs, ts)
+g.replay()
+torch.cuda.synchronize()
+assert c.lens.tolist() == [300, 300]
+assert all(torch.equal(a, c.attend(0, x)) for a, x in zip(got, q)) and torch.equal(v[0], c.read(300)[0]) and (y == 0).all()
+print("captured first")
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_of_a_process_may_be_captured(require_gpu):
+    """Kernels are loaded, limits set and the device's room asked for inside the capture."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert "captured first" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_calls_from_several_threads(require_gpu):
+    """Two caches, a thread and a stream each, long enough to overlap: the results of calls one after the other."""
+    from flashact_b200 import Kv8Cache
+    g = torch.Generator().manual_seed(8)
+    work, want = [], []
+    for n in (700, 9000):
+        c = Kv8Cache(3, 1, 2, 128, 1 << 14)
+        k = torch.randn(3, n, 2, 128, generator=g).to(BF).cuda()
+        c.append(0, k, k)
+        c.advance(n)
+        qs = [torch.randn(3, t, 8, 128, generator=g).to(dt).cuda() for t in (1, 3, 30) for dt in (BF, HF)]
+        work.append((c, qs))
+        want.append([c.attend(0, q) for q in qs])
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        try:
+            c, qs = work[i]
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(60):
+                    got = [c.attend(0, q) for q in qs]
+                torch.cuda.current_stream().synchronize()
+                bad.extend(j for j, (a, b) in enumerate(zip(got, want[i])) if not torch.equal(a, b))
+        except Exception as e:  # noqa: BLE001
+            bad.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
