@@ -49,8 +49,10 @@ def bind_cache(engine, bind, cache, want, valid_len, stream):
         valid_len = [int(x) for x in valid_len]
         if len(valid_len) != cache.batch or min(valid_len) < 0 or max(valid_len) > cache.capacity:
             raise C.FlashActError(C.FA_ERR_INVALID, f"lengths {valid_len} for a cache of {cache.batch} x {cache.capacity} tokens")
-        lens = torch.tensor(valid_len, dtype=torch.int32, device=cache.device)  # what is bound is what is read, whatever cache.lens says
-        k, v = cache.read(max(1, max(valid_len)), lens=lens)
+        # every row up to the longest, whatever cache.lens says: the bind takes valid_len of them and clears the rest itself. A fill, not a
+        # copy from the host: a bind with the lengths of the last one waits for nothing and can be captured.
+        rows = max(1, max(valid_len))
+        k, v = cache.read(rows, lens=torch.full((cache.batch,), rows, dtype=torch.int32, device=cache.device))
         bind(k, v, valid_len)
 
 

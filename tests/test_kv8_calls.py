@@ -382,3 +382,30 @@ def test_calls_from_several_threads(require_gpu):
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.gpu
+def test_bind_with_the_same_lengths_may_be_captured(require_gpu):
+    """Lengths that the host knows cost no copy to the device and no wait: a bind with those of the last one is launches alone."""
+    from flashact_b200 import Kv8Cache
+    from oracle import pi05_oracle as O
+    from tests.pi05_util import engine_for
+    c = O.make_case(seed=9, L=2, T=50, AD=32, Lp=64, B=2, num_steps=2)
+    eng, cache = engine_for(c), Kv8Cache(2, 2, 1, 256, 64)
+
+    def fill(scale):
+        for layer in range(2):
+            cache.append(layer, (c.k[:, layer, :, None] * scale).contiguous().cuda(), (c.v[:, layer, :, None] * scale).contiguous().cuda())
+    fill(1.0)
+    eng.bind_prefix_cache(cache, [64, 40])
+    first = eng.sample_actions(c.noise.cuda())
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        eng.bind_prefix_cache(cache, [64, 40])
+    fill(0.5)
+    g.replay()
+    got = eng.sample_actions(c.noise.cuda())
+    eng.bind_prefix_cache(cache, [64, 40])
+    assert torch.equal(got, eng.sample_actions(c.noise.cuda())) and not torch.equal(got, first)
+    eng.close()
