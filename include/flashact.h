@@ -185,23 +185,24 @@ FA_API fa_status fa_kv8_append(const fa_kv8* c, int layer, int rows, const fa_ro
 FA_API fa_status fa_kv8_read(const fa_kv8* c, const int* lens, int rows, void* k, void* v, fa_dtype dtype,
                              fa_stream stream);
 
-/* Attention of `tokens` query tokens over layer `layer`: out = softmax(scale q K^T + mask) V, rounded once to the queries' type
- * (`dtype`: bf16 or f16). Scores, maxima and sums are fp32; what goes into the products has fewer bits than that: a probability
- * times its V scale is off by at most 2^-11 of itself (f16 queries 2^-15) and by 2^-29 of the largest such product that the row sees,
- * and an element of a query by 2^-17 of the row's largest element (2^-21 with up to 16 query rows of a key head). q and out are [batch][tokens][q_heads][head_dim] rows; out may be q
- * (the same pointer and strides), but for that its rows overlap neither q nor one another; query head
- * i reads key head i / (q_heads / heads). lens, q_lens, prefix: device int32 [batch]. lens[b] tokens
- * of observation b are in the cache, the queries' own included where they attend to themselves; q_lens[b] (NULL:
- * tokens) of its query tokens are real: the output rows of the others are left as they were. Query token i
- * stands at position lens[b] - q_lens[b] + i. causal: it sees the keys up to its position, and all below prefix[b] (NULL: 0); not
- * causal: all lens[b]. A query that sees no key gets zeros. max_len is an upper bound of lens known to the host
- * (0: capacity); lengths above it count as it. The work is split by max_len, and the splits are joined in a fixed
- * order: results do not depend on timing. workspace: fa_kv8_attention_workspace bytes, 16-byte aligned,
- * nothing kept in it between calls; calls that overlap on the GPU need one each. The need follows the splits and does not grow with the
- * sizes: one token over a long cache may need more than a prompt, which needs none. One workspace for several calls is the
- * largest of what each of their (cache, tokens, q_heads, max_len) asks for. Codes behind lens[b]
- * may hold anything; a NaN code before it makes the result of its head NaN, masked or not. Each wait on the device is bounded; one that
- * runs out, which no input brings about, is seen in the result, not in the status: the query rows that it served are NaN. */
+/* Attention of `tokens` query tokens over layer `layer`: out = softmax(scale q K^T + mask) V, rounded once to the
+ * queries' type (`dtype`: bf16 or f16). Scores, maxima and sums are fp32; what goes into the products has fewer bits
+ * than that: a probability times its V scale is off by at most 2^-11 of itself (f16 queries 2^-15) and by 2^-29 of the
+ * largest such product that the row sees, and an element of a query by 2^-17 of the row's largest element (2^-21 with up
+ * to 16 query rows of a key head). q and out are [batch][tokens][q_heads][head_dim] rows; out may be q (the same pointer
+ * and strides), but for that its rows overlap neither q nor one another; query head i reads key head i / (q_heads /
+ * heads). lens, q_lens, prefix: device int32 [batch]. lens[b] tokens of observation b are in the cache, the queries' own
+ * included where they attend to themselves; q_lens[b] (NULL: tokens) of its query tokens are real: the output rows of
+ * the others are left as they were. Query token i stands at position lens[b] - q_lens[b] + i. causal: it sees the keys
+ * up to its position, and all below prefix[b] (NULL: 0); not causal: all lens[b]. A query that sees no key gets zeros.
+ * max_len is an upper bound of lens known to the host (0: capacity); lengths above it count as it. The work is split by
+ * max_len, and the splits are joined in a fixed order: results do not depend on timing. workspace:
+ * fa_kv8_attention_workspace bytes, 16-byte aligned, nothing kept in it between calls; calls that overlap on the GPU
+ * need one each. The need follows the splits and does not grow with the sizes: one token over a long cache may need more
+ * than a prompt, which needs none. One workspace for several calls is the largest of what each of their (cache, tokens,
+ * q_heads, max_len) asks for. Codes behind lens[b] may hold anything; a NaN code before it makes the result of its head
+ * NaN, masked or not. Each wait on the device is bounded; one that runs out, which no input brings about, is seen in the
+ * result, not in the status: the query rows that it served are NaN. */
 FA_API fa_status fa_kv8_attention_workspace(const fa_kv8* c, int tokens, int q_heads, int max_len, size_t* bytes);
 FA_API fa_status fa_kv8_attention(const fa_kv8* c, int layer, int tokens, int q_heads, const fa_rows* q, fa_dtype dtype,
                                   const int* lens, const int* q_lens, const int* prefix, int causal, float scale,
