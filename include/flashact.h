@@ -147,7 +147,7 @@ FA_API fa_status fa_nvfp4_linear(const void* x, fa_dtype dtype, int M, int K, lo
 
 /* ---- 8-bit KV cache ----
  * The keys and values of a prefix in E4M3 with one fp32 scale for each block of `block` tokens and head: half the
- * bytes of the bf16 prefix. value = code x scale of its block. K is kept token by token, V transposed (both
+ * bytes of the bf16 prefix. value = code x scale of its block, a positive finite number. K is kept token by token, V transposed (both
  * then feed the attention's products along contiguous bytes).
  *   k       [batch][layers][heads][capacity][head_dim] codes
  *   v       [batch][layers][heads][head_dim][capacity] codes
@@ -200,7 +200,7 @@ FA_API fa_status fa_kv8_read(const fa_kv8* c, const int* lens, int rows, void* k
  * fa_kv8_attention_workspace bytes, 16-byte aligned, nothing kept in it between calls; calls that overlap on the GPU
  * need one each. The need follows the splits and does not grow with the sizes: one token over a long cache may need more
  * than a prompt, which needs none. One workspace for several calls is the largest of what each of their (cache, tokens,
- * q_heads, max_len) asks for. Codes behind lens[b] may hold anything; a NaN code before it makes the result of its head
+ * q_heads, max_len) asks for, on the device of the calls: the splits go by what it has room for. Codes behind lens[b] may hold anything; a NaN code before it makes the result of its head
  * NaN, masked or not. Each wait on the device is bounded; one that runs out, which no input brings about, is seen in the
  * result, not in the status: the query rows that it served are NaN. */
 FA_API fa_status fa_kv8_attention_workspace(const fa_kv8* c, int tokens, int q_heads, int max_len, size_t* bytes);
